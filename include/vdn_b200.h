@@ -389,6 +389,54 @@ int vdn_vda_forward_noalloc(const void* q, const void* k, const void* v, int64_t
                             const int32_t* bounds, const float* seed, int bridge,
                             int F, int S, int H, int d, void* out, cudaStream_t stream);
 
+/* ------------------------------------------- differentiable operators (per token) */
+
+/* Gated linear recurrence, per channel: h_t = exp(log_decay_t) h_{t-1} + x_t, y_t = h_t.
+ * Dense: x is [seqs, rows, heads * d] (batch and row strides in elements, channels
+ * contiguous); packed (cu_seqlens != NULL): [rows, heads * d], sequence s holding rows
+ * cu_seqlens[s] .. cu_seqlens[s + 1] (device int32, nondecreasing, clamped to [0, rows];
+ * empty sequences allowed).  reverse: each sequence runs from its last row to its first.
+ * dtype: x and y; g_dtype: log_decay, the same or fp32.  shared: one decay per head
+ * ([.., heads], d 32, 64 or 128).  state / out_state: fp32 [seqs, heads * d] or NULL (zeros
+ * in / not wanted); out_state may be state.  zero_tail: write zeros to the rows behind the
+ * last packed sequence, else they are left alone.  rows and channels below 2^30, row strides
+ * below 2^26.  States and sums are fp32 and added in a fixed order.  status: as in vdn_mxfp8_gemm.
+ * Per-token companion of the frame-wise scan, src/models/linear_attention/scan.py:270-355. */
+int vdn_gated_scan(const void* x, int dtype, int64_t x_batch, int64_t x_row, const void* log_decay,
+                   int g_dtype, int64_t g_batch, int64_t g_row, int shared, const float* state,
+                   const int32_t* cu_seqlens, int64_t seqs, int64_t rows, int64_t heads, int64_t d,
+                   int reverse, void* y, int64_t y_batch, int64_t y_row, int zero_tail,
+                   float* out_state, int* status, cudaStream_t stream);
+
+/* Gradients of vdn_gated_scan from dy and d_out_state (or NULL): dx (dtype), dg (g_dtype,
+ * summed over the head when shared) and d_state (fp32, or NULL).  y is the forward's
+ * output, state its first state.  dx and dg must not overlap the inputs. */
+int vdn_gated_scan_backward(const void* dy, int dtype, int64_t dy_batch, int64_t dy_row,
+                            const void* log_decay, int g_dtype, int64_t g_batch, int64_t g_row,
+                            int shared, const void* y, int64_t y_batch, int64_t y_row,
+                            const float* state, const float* d_out_state, const int32_t* cu_seqlens,
+                            int64_t seqs, int64_t rows, int64_t heads, int64_t d, int reverse, void* dx,
+                            int64_t dx_batch, int64_t dx_row, void* dg, int64_t dg_batch,
+                            int64_t dg_row, int zero_tail, float* d_state, int* status,
+                            cudaStream_t stream);
+
+/* Layer norm over the last dimension: y = (x - mean) * rstd * weight + bias, with
+ * rstd = 1 / sqrt(var + eps).  x, y [rows, width] of `dtype` (row strides in elements);
+ * weight, bias [width] of w_dtype (dtype or fp32), either may be NULL; mean, rstd fp32
+ * [rows], optional outputs. */
+int vdn_layer_norm(const void* x, int dtype, int64_t rows, int64_t width, int64_t x_stride,
+                   const void* weight, const void* bias, int w_dtype, float eps, void* y,
+                   int64_t y_stride, float* mean, float* rstd, cudaStream_t stream);
+
+/* Gradients of vdn_layer_norm: dx (dtype), d_weight and d_bias (w_dtype, either may be
+ * NULL), the two summed over the rows in fp32 and in a fixed order through the workspace. */
+size_t vdn_layer_norm_backward_workspace_size(int64_t rows, int64_t width);
+int vdn_layer_norm_backward(const void* dy, int dtype, int64_t rows, int64_t width, int64_t dy_stride,
+                            const void* x, int64_t x_stride, const void* weight, int w_dtype,
+                            const float* mean, const float* rstd, void* dx, int64_t dx_stride,
+                            void* d_weight, void* d_bias, void* workspace, size_t workspace_bytes,
+                            cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

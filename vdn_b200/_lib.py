@@ -74,6 +74,15 @@ SIGNATURES = {
                                _p, _p, _i32, _i32, _i32, _i32, _i32, _p, _p, _sz, _p]),
     "vdn_vda_forward_noalloc": (_i32, [_p, _p, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p,
                                        _f32, _p, _p, _i32, _i32, _i32, _i32, _i32, _p, _p]),
+    "vdn_gated_scan": (_i32, [_p, _i32, _i64, _i64, _p, _i32, _i64, _i64, _i32, _p, _p, _i64, _i64, _i64, _i64,
+                              _i32, _p, _i64, _i64, _i32, _p, _p, _p]),
+    "vdn_gated_scan_backward": (_i32, [_p, _i32, _i64, _i64, _p, _i32, _i64, _i64, _i32, _p, _i64, _i64, _p, _p,
+                                       _p, _i64, _i64, _i64, _i64, _i32, _p, _i64, _i64, _p, _i64, _i64, _i32,
+                                       _p, _p, _p]),
+    "vdn_layer_norm": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _p, _i32, _f32, _p, _i64, _p, _p, _p]),
+    "vdn_layer_norm_backward_workspace_size": (_sz, [_i64, _i64]),
+    "vdn_layer_norm_backward": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _i32, _p, _p, _p, _i64, _p, _p,
+                                       _p, _sz, _p]),
 }
 
 _LOCK = threading.Lock()
@@ -102,6 +111,23 @@ def call(name: str, *args) -> int:
     if rc != VDN_OK:
         raise_status(rc)
     return rc
+
+
+def call_on(device: torch.device, name: str, *args) -> int:
+    """call(name, *args, stream) on `device`'s current stream, with `device` current."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return call(name, *args, stream_of(device))
+    return call(name, *args, stream_of(device))
+
+
+def refuse_captured_autograd(name: str) -> None:
+    """A recorded graph must not span a stream capture: the engine runs the gradient
+    accumulators of leaves that an eager graph still holds on that graph's stream, which is
+    not being captured.  So the differentiable ops refuse to record while capturing."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{name} does not record gradients during stream capture; capture the explicit "
+                           f"forward and {name}_backward calls instead")
 
 
 def raise_status(rc: int):
