@@ -39,10 +39,12 @@ extern "C" {
 #define VDN_DTYPE_BF16 1
 #define VDN_DTYPE_F16 2
 
-/* Activations of vdn_mxfp8_act_quantize. */
+/* Activations of vdn_mxfp8_act_quantize (1..3) and vdn_linear_act (all but SWIGLU). */
+#define VDN_ACT_NONE 0
 #define VDN_ACT_GELU_TANH 1
 #define VDN_ACT_GELU_ERF 2
 #define VDN_ACT_SWIGLU 3
+#define VDN_ACT_SILU 4
 
 /* Message of the last failing call on this thread ("" if none). */
 const char* vdn_last_error(void);
@@ -436,6 +438,32 @@ int vdn_layer_norm_backward(const void* dy, int dtype, int64_t rows, int64_t wid
                             const float* mean, const float* rstd, void* dx, int64_t dx_stride,
                             void* d_weight, void* d_bias, void* workspace, size_t workspace_bytes,
                             cudaStream_t stream);
+
+/* Linear layer on tcgen05, 16-bit operands (`dtype` bf16 or fp16, all matrices alike), fp32
+ * accumulation: z = x w^T + bias, pre = z (if not NULL), y = act(z) + residual (if not
+ * NULL).  x [rows, k] and w [n, k] 16-byte aligned with row strides multiples of 8
+ * elements; bias [n], residual, y and pre [rows, n] with any row stride.  y must not
+ * overlap the inputs.  act: VDN_ACT_NONE, _GELU_TANH, _GELU_ERF or _SILU.  status: as in
+ * vdn_mxfp8_gemm.  The 16-bit, trainable counterpart of the block's MXFP8 projections with
+ * fused epilogues (src/models/ops/mxfp8_linear.py:60-102). */
+int vdn_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
+                   const void* residual, int64_t ldr, int dtype, int act, int64_t rows, int64_t n,
+                   int64_t k, void* y, int64_t ldy, void* pre, int64_t ldp, int* status,
+                   cudaStream_t stream);
+
+/* dz = dy act'(pre) [rows, n] (nothing is written for VDN_ACT_NONE: dz is dy) and d_bias [n]
+ * (or NULL) = its column sums, in fp32 and a fixed order through the workspace. */
+size_t vdn_linear_dz_workspace_size(int64_t rows, int64_t n);
+int vdn_linear_dz(const void* dy, int64_t ldy, const void* pre, int64_t ldp, int dtype, int act,
+                  int64_t rows, int64_t n, void* dz, int64_t ldz, void* d_bias, void* workspace,
+                  size_t workspace_bytes, cudaStream_t stream);
+
+/* dx [rows, k] = dz [rows, n] w [n, k], and dw [n, k] = dz^T x [rows, k].  dz, w and x as the
+ * operands of vdn_linear_act, the outputs with any row stride. */
+int vdn_linear_dx(const void* dz, int64_t ldz, const void* w, int64_t ldw, int dtype, int64_t rows,
+                  int64_t n, int64_t k, void* dx, int64_t ldx, int* status, cudaStream_t stream);
+int vdn_linear_dw(const void* dz, int64_t ldz, const void* x, int64_t ldx, int dtype, int64_t rows,
+                  int64_t n, int64_t k, void* dw, int64_t ldw, int* status, cudaStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -18,7 +18,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libvdn_b200.so"
 
 VDN_OK, VDN_ERR_VALUE, VDN_ERR_TYPE, VDN_ERR_RUNTIME, VDN_ERR_NONFINITE, VDN_ERR_TIMEOUT = range(6)
 DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
-ACT_GELU_TANH, ACT_GELU_ERF, ACT_SWIGLU = 1, 2, 3
+ACT_NONE, ACT_GELU_TANH, ACT_GELU_ERF, ACT_SWIGLU, ACT_SILU = range(5)
 
 _i64, _i32, _f32, _sz = C.c_int64, C.c_int, C.c_float, C.c_size_t
 _p = C.c_void_p
@@ -83,6 +83,12 @@ SIGNATURES = {
     "vdn_layer_norm_backward_workspace_size": (_sz, [_i64, _i64]),
     "vdn_layer_norm_backward": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _i32, _p, _p, _p, _i64, _p, _p,
                                        _p, _sz, _p]),
+    "vdn_linear_act": (_i32, [_p, _i64, _p, _i64, _p, _p, _i64, _i32, _i32, _i64, _i64, _i64, _p, _i64, _p, _i64,
+                              _p, _p]),
+    "vdn_linear_dz_workspace_size": (_sz, [_i64, _i64]),
+    "vdn_linear_dz": (_i32, [_p, _i64, _p, _i64, _i32, _i32, _i64, _i64, _p, _i64, _p, _p, _sz, _p]),
+    "vdn_linear_dx": (_i32, [_p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _p, _i64, _p, _p]),
+    "vdn_linear_dw": (_i32, [_p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _p, _i64, _p, _p]),
 }
 
 _LOCK = threading.Lock()

@@ -338,28 +338,6 @@ __global__ void __launch_bounds__(256) columns_wide_kernel(const Bwd p) {
   part[p.width + c] = db;
 }
 
-// dw[c], db[c] = the lines' sums in a fixed order: 32 columns by 8 line groups a block.
-template <typename TW>
-__global__ void __launch_bounds__(256) lines_kernel(const float* part, int lines, int width, TW* dw, TW* db) {
-  __shared__ float sums[8][33];
-  const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;   // of 2 * width columns
-  float s = 0.f;
-  if (c < 2 * (int64_t)width)
-    for (int l = g; l < lines; l += 8) s += part[(int64_t)l * 2 * width + c];
-  sums[g][lane] = s;
-  __syncthreads();
-  if (g == 0 && c < 2 * (int64_t)width) {
-#pragma unroll
-    for (int k = 1; k < 8; ++k) s += sums[k][lane];
-    if (c < width) {
-      if (dw) dw[c] = from_f32<TW>(s);
-    } else if (db) {
-      db[c - width] = from_f32<TW>(s);
-    }
-  }
-}
-
 template <typename T, typename TW, int VEC, int NV, int LANES, int MAXT>
 static int launch_forward(const Fwd& p, int block, cudaStream_t stream) {
   const int64_t per = LANES ? block / (LANES ? LANES : 1) : 1;
@@ -431,12 +409,8 @@ static int backward(const Bwd& p, int lines, void* dw, void* db, cudaStream_t st
     columns_wide_kernel<T><<<dim3((p.width + 255) / 256, lines), 256, 0, stream>>>(p);
     VDN_LAUNCH_CHECK("layer norm backward (wide columns)");
   }
-  if (dw || db) {
-    lines_kernel<TW><<<(unsigned)((2 * (int64_t)p.width + 31) / 32), 256, 0, stream>>>(
-        p.part, lines, p.width, static_cast<TW*>(dw), static_cast<TW*>(db));
-    VDN_LAUNCH_CHECK("layer norm backward (line sums)");
-  }
-  return VDN_OK;
+  if (!dw && !db) return VDN_OK;
+  return add_lines<TW>(p.part, lines, 2 * (int64_t)p.width, static_cast<TW*>(dw), p.width, static_cast<TW*>(db), stream);
 }
 
 static int check(int dtype, int w_dtype, int64_t rows, int64_t width) {

@@ -5,6 +5,8 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace vdn {
@@ -48,13 +50,35 @@ template <typename R> __device__ __forceinline__ void store_once(void* p, const 
 
 inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
-// Calls f with a value of the element type of a VDN_DTYPE code.
-#define VDN_BY_DTYPE(code, T, ...)                              \
-  switch (code) {                                               \
-    case VDN_DTYPE_F32: { using T = float; __VA_ARGS__; break; }         \
-    case VDN_DTYPE_BF16: { using T = __nv_bfloat16; __VA_ARGS__; break; } \
-    default: { using T = __half; __VA_ARGS__; break; }          \
+// Sums `lines` lines of `cols` fp32 partial sums in a fixed order: 32 columns by 8 line
+// groups a block.  Columns below `split` go to `a`, the others to `b` (either may be null).
+template <typename T>
+__global__ void __launch_bounds__(256) lines_kernel(const float* part, int lines, int64_t cols, T* a, int64_t split,
+                                                    T* b) {
+  __shared__ float sums[8][33];
+  const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  float s = 0.f;
+  if (c < cols)
+    for (int l = g; l < lines; l += 8) s += part[l * cols + c];
+  sums[g][lane] = s;
+  __syncthreads();
+  if (g == 0 && c < cols) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += sums[k][lane];
+    if (c < split) {
+      if (a) a[c] = from_f32<T>(s);
+    } else if (b) {
+      b[c - split] = from_f32<T>(s);
+    }
   }
+}
+template <typename T>
+inline int add_lines(const float* part, int lines, int64_t cols, T* a, int64_t split, T* b, cudaStream_t stream) {
+  lines_kernel<T><<<(unsigned)((cols + 31) / 32), 256, 0, stream>>>(part, lines, cols, a, split, b);
+  VDN_LAUNCH_CHECK("line sums");
+  return VDN_OK;
+}
 
 inline int dtype_bytes(int code) { return code == VDN_DTYPE_F32 ? 4 : 2; }
 inline bool dtype_known(int code) { return code == VDN_DTYPE_F32 || code == VDN_DTYPE_BF16 || code == VDN_DTYPE_F16; }

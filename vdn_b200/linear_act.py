@@ -1,0 +1,166 @@
+"""Linear layer with bias, activation and residual in one kernel, with its gradients.
+
+    y = act(x @ weight.T + bias) + residual        act: none, gelu_tanh, gelu_erf, silu
+
+in bf16 or fp16 on tcgen05 with fp32 accumulation (vdn_linear_act): the trainable 16-bit
+counterpart of the block's MXFP8 projections and their fused epilogues
+(src/models/ops/mxfp8_linear.py:60-102).  The activation and the residual add work on the
+fp32 sum; y is rounded once.
+
+Differentiable: with gradients enabled, linear_act records itself for autograd; the same
+backward is public as linear_act_backward (the form to capture into a CUDA graph).
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .mxfp8_linear import _status
+
+__all__ = ["linear_act", "linear_act_backward", "ACTIVATIONS"]
+
+ACTIVATIONS = {"none": _lib.ACT_NONE, "gelu_tanh": _lib.ACT_GELU_TANH, "gelu_erf": _lib.ACT_GELU_ERF,
+               "silu": _lib.ACT_SILU}
+
+
+def _pad8(n):
+    return (n + 7) // 8 * 8
+
+
+def _operand(t):
+    """t [rows, cols] as the tensor maps take it: unit column stride, 16-byte aligned rows
+    (copied into padded rows where its layout does not suit them)."""
+    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
+        return t
+    return torch.empty(t.shape[0], _pad8(t.shape[1]), dtype=t.dtype, device=t.device)[:, :t.shape[1]].copy_(t)
+
+
+def _matrix(t, cols):
+    """t [..., cols] as [rows, cols] with unit column stride (any row stride)."""
+    flat = t.reshape(-1, cols)
+    return flat if flat.stride(1) == 1 or cols == 1 else flat.contiguous()
+
+
+def _check(x, weight, act):
+    if not isinstance(x, torch.Tensor) or not isinstance(weight, torch.Tensor):
+        raise TypeError("x and weight must be tensors")
+    if x.dtype not in (torch.bfloat16, torch.float16) or weight.dtype != x.dtype:
+        raise TypeError(f"x and weight must both be bf16 or both fp16, got {x.dtype} and {weight.dtype}")
+    if not x.is_cuda or weight.device != x.device:
+        raise ValueError("x and weight must be CUDA tensors on one device")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError("x must be [..., k] and weight [n, k]")
+    if weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError("weight must not be empty")
+    if act not in ACTIVATIONS:
+        raise ValueError(f"act must be one of {tuple(ACTIVATIONS)}, got {act!r}")
+    _lib.require_device(x, "x")
+
+
+def _same(t, x, shape, name):
+    if t.dtype != x.dtype or t.device != x.device:
+        raise TypeError(f"{name} must have x's dtype and device")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+
+
+def _forward(x, weight, bias, act, residual, want_pre):
+    _check(x, weight, act)
+    n, k = weight.shape
+    shape = (*x.shape[:-1], n)
+    if bias is not None:
+        _same(bias, x, (n,), "bias")
+        bias = bias.contiguous()
+    if residual is not None:
+        _same(residual, x, shape, "residual")
+    flat = _operand(x.reshape(-1, k))
+    w = _operand(weight)
+    rows = flat.shape[0]
+    res = None if residual is None else _matrix(residual, n)
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    pre = torch.empty(shape, dtype=x.dtype, device=x.device) if want_pre else None
+    _lib.call_on(x.device, "vdn_linear_act", flat.data_ptr(), flat.stride(0), w.data_ptr(), w.stride(0),
+                 _lib.ptr(bias), _lib.ptr(res), res.stride(0) if res is not None else 0, _lib.dtype_code(x.dtype),
+                 ACTIVATIONS[act], rows, n, k, y.data_ptr(), n, _lib.ptr(pre), n, _status(x.device).data_ptr())
+    return y, pre
+
+
+class _LinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, act, residual):
+        y, pre = _forward(x, weight, bias, act, residual, act != "none")
+        ctx.save_for_backward(x, weight, pre)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y):
+        x, weight, pre = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw, db = _backward(grad_y, x, weight, pre, ctx.act, need[0], need[1], need[2])
+        return dx, dw, db, None, grad_y if need[4] else None
+
+
+def linear_act(x, weight, bias=None, *, act="none", residual=None, return_pre=False):
+    """act(x @ weight.T + bias) + residual for x [..., k], weight [n, k], bias [n] and residual
+    [..., n], all bf16 or all fp16; act is one of ACTIVATIONS.  With return_pre also
+    x @ weight.T + bias, rounded (what linear_act_backward takes for an activation).
+
+    Row-strided operands are read in place where their rows are 16-byte aligned, others
+    (odd k, transposed) are copied into padded rows first."""
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
+                                       for t in (x, weight, bias, residual)):
+        if return_pre:
+            raise ValueError("return_pre is for the explicit backward, not where gradients are recorded")
+        _lib.refuse_captured_autograd("linear_act")
+        return _LinearAct.apply(x, weight, bias, act, residual)
+    y, pre = _forward(x, weight, bias, act, residual, return_pre)
+    return (y, pre) if return_pre else y
+
+
+def _backward(grad_y, x, weight, pre, act, want_x, want_w, want_b):
+    _check(x, weight, act)
+    n, k = weight.shape
+    shape = (*x.shape[:-1], n)
+    _same(grad_y, x, shape, "grad_y")
+    if act != "none":
+        if pre is None:
+            raise ValueError("pre (linear_act's return_pre) is needed for the activation's gradient")
+        _same(pre, x, shape, "pre")
+    dev, code, word = x.device, _lib.dtype_code(x.dtype), _status(x.device).data_ptr()
+    dy = _matrix(grad_y, n)
+    rows = dy.shape[0]
+    db = torch.empty(n, dtype=x.dtype, device=dev) if want_b else None
+    need = _lib.load().vdn_linear_dz_workspace_size(rows, n) if want_b else 0
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if want_b else None
+    dz, z = dy, None
+    if act != "none":
+        z = _matrix(pre, n)
+        dz = torch.empty(rows, _pad8(n), dtype=x.dtype, device=dev)[:, :n]
+    if want_b or act != "none":
+        _lib.call_on(dev, "vdn_linear_dz", dy.data_ptr(), dy.stride(0), _lib.ptr(z), z.stride(0) if z is not None else 0,
+                     code, ACTIVATIONS[act], rows, n, dz.data_ptr(), dz.stride(0), _lib.ptr(db), _lib.ptr(ws), need)
+    dx = dw = None
+    if want_x or want_w:
+        dz = _operand(dz)
+    if want_x:
+        w = _operand(weight)
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        _lib.call_on(dev, "vdn_linear_dx", dz.data_ptr(), dz.stride(0), w.data_ptr(), w.stride(0), code, rows, n, k,
+                     dx.data_ptr(), k, word)
+    if want_w:
+        flat = _operand(x.reshape(-1, k))
+        dw = torch.empty(n, k, dtype=x.dtype, device=dev)
+        _lib.call_on(dev, "vdn_linear_dw", dz.data_ptr(), dz.stride(0), flat.data_ptr(), flat.stride(0), code, rows, n,
+                     k, dw.data_ptr(), k, word)
+    return dx, dw, db
+
+
+@torch.no_grad()
+def linear_act_backward(grad_y, x, weight, pre=None, *, act="none", bias=True):
+    """(grad of x, of weight, of bias or None) from the forward's inputs and `pre`.  The residual's
+    gradient is grad_y.  The activation's gradient enters the two products rounded to the
+    operands' type; the bias gradient sums it unrounded, in fp32 and a fixed order."""
+    return _backward(grad_y, x, weight, pre, act, True, True, bool(bias))
