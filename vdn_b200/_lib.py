@@ -119,12 +119,37 @@ def call(name: str, *args) -> int:
     return rc
 
 
-def call_on(device: torch.device, name: str, *args) -> int:
-    """call(name, *args, stream) on `device`'s current stream, with `device` current."""
-    if device.index != torch.cuda.current_device():
+_FUNCTIONS: dict[str, object] = {}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """The entry point `name` with `device` current and its current stream as last argument
+    (pointers as plain addresses: the short path of the ops whose calls cost microseconds)."""
+    fn = _FUNCTIONS.get(name)
+    if fn is None:
+        fn = _FUNCTIONS[name] = getattr(load(), name)
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
+    else:
         with torch.cuda.device(device):
-            return call(name, *args, stream_of(device))
-    return call(name, *args, stream_of(device))
+            rc = fn(*args, _raw_stream(index))
+    if rc != VDN_OK:
+        raise_status(rc)
+
+
+def records(*tensors) -> bool:
+    """Whether any of the arguments (tensors or None) asks for gradients."""
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
+
+
+def address(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
 
 
 def refuse_captured_autograd(name: str) -> None:
@@ -170,8 +195,11 @@ def require_device(t: torch.Tensor, what: str = "tensor") -> None:
         raise RuntimeError("vdn_b200 kernels require an sm_100 (B200) GPU; no fallback")
 
 
+_DTYPE_CODES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
+
+
 def dtype_code(dtype: torch.dtype) -> int:
     try:
-        return {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}[dtype]
+        return _DTYPE_CODES[dtype]
     except KeyError:
         raise TypeError(f"unsupported dtype {dtype}") from None

@@ -97,6 +97,7 @@ struct Params {
   int64_t rows, cols, ldr, ldy, ldp;
   int m_tiles, n_tiles, k_blocks;
   bool tma_y, tma_p, tma_r;   // alignment allows bulk stores / loads of that matrix
+  bool bias_vec;
   int* status;
 };
 
@@ -320,12 +321,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
           }
         }
         if (!live) continue;
-        if (p.bias) {
+        if (p.bias) {                                    // the same address in every lane: one broadcast each
           const T* bias = static_cast<const T*>(p.bias) + col0;
+          if (p.bias_vec && col0 + 64 <= p.cols) {
 #pragma unroll
-          for (int c = 0; c < 64; ++c) {
-            const float add = col0 + c < p.cols ? to_f32(bias[c]) : 0.f;
-            r[c] = __float_as_uint(__uint_as_float(r[c]) + add);
+            for (int c = 0; c < 8; ++c) {
+              float e[8];
+              unpack<T, 8>(__ldg(reinterpret_cast<const uint4*>(bias) + c), e);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) r[8 * c + i] = __float_as_uint(__uint_as_float(r[8 * c + i]) + e[i]);
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < 64; ++c)
+              if (col0 + c < p.cols) r[c] = __float_as_uint(__uint_as_float(r[c]) + to_f32(bias[c]));
           }
         }
         auto put = [&](auto value) {                     // 64 results of this row, rounded, to the piece
@@ -406,27 +415,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 }
 
 // ---------------------------------------------------------------- narrow kernel
-constexpr int NARROW_THREADS = 192;
+constexpr int NARROW_THREADS = 320;          // producer, issuer, eight epilogue warps
 template <int BN> constexpr int narrow_stages() { return BN >= 128 ? 3 : BN >= 64 ? 4 : BN >= 32 ? 5 : 6; }   // two CTAs an SM
 template <int BN> constexpr size_t narrow_ring() { return narrow_stages<BN>() * (size_t)(16384 + BN * 128); }
 template <int BN> constexpr size_t narrow_smem() { return 1024 + narrow_ring<BN>() + 256; }
 static_assert(narrow_smem<16>() <= 115712 && narrow_smem<32>() <= 115712 && narrow_smem<64>() <= 115712 &&
               narrow_smem<128>() <= 115712, "two CTAs an SM");
 
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
+// Each thread of the warp reads N columns of its TMEM lane.
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_32x32b_x32(taddr, r); }
+
+__device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
 // D^T: features (the output's columns) on M, tokens (its rows) on N.  m_tiles counts
-// 128-feature tiles, n_tiles BN-token tiles; the cluster's CTAs share one tile's depth.
+// 128-feature tiles, n_tiles BN-token tiles; the cluster's CTAs share one tile's depth, and
+// CTA r finishes the r-th part of its tokens from the parts that all CTAs push to it.
 template <typename T, bool F_MN, bool X_MN, int ACT, int BN>
 __global__ void __launch_bounds__(NARROW_THREADS, 2)
     narrow_kernel(const __grid_constant__ CUtensorMap tf, const __grid_constant__ CUtensorMap tx, const Params p,
                   const int split) {
   constexpr int ST = narrow_stages<BN>(), A_BYTES = 16384, B_BYTES = BN * 128;
-  constexpr int COLS = BN < 32 ? 32 : BN;
+  constexpr int COLS = BN < 32 ? 32 : BN;    // TMEM columns
+  constexpr int CH = BN / 2 < 32 ? BN / 2 : 32;   // tokens an epilogue warp holds at a time
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -436,7 +460,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 2)
   uint64_t* acc_full = empty + ST;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  float* parts = reinterpret_cast<float*>(smem);         // [BN][128] after the ring is done
+  float* parts = reinterpret_cast<float*>(smem);   // [source rank][token of this CTA][128], in the idle ring
   static_assert(BN * 128 * 4 <= narrow_ring<BN>(), "parts fit the ring");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -452,8 +476,6 @@ __global__ void __launch_bounds__(NARROW_THREADS, 2)
     mbar_init(acc_full, 1);
     *abort_flag = 0;
     fence_barrier_init();
-    prefetch_tensormap(&tf);
-    prefetch_tensormap(&tx);
   }
   if (warp == 1) tmem_alloc(tmem_holder, COLS);
   tc_fence_before();
@@ -500,7 +522,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 2)
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      constexpr uint32_t kIdesc = idesc_f16<T>(128, BN, F_MN, X_MN);
+      constexpr uint32_t kIdesc = idesc_f16<T>(128, BN, F_MN, X_MN);   // kind::f16, the type in the descriptor
       int stage = 0;
       uint32_t phase = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
@@ -520,68 +542,85 @@ __global__ void __launch_bounds__(NARROW_THREADS, 2)
     }
   }
   __syncwarp();                              // no lane spins beside its warp's producer or issuer
+  const bool epi = warp >= 2;
+  const int quad = warp & 3, group = (warp - 2) >> 2;   // TMEM lane quadrant, half of the tokens
+  const int f = quad * 32 + lane;            // feature within the tile
+  const int64_t col = (int64_t)ft * 128 + f;
+  const bool in = epi && col < p.cols;
+  const float bias = in && p.bias ? to_f32(static_cast<const T*>(p.bias)[col]) : 0.f;
+  const int64_t row0 = (int64_t)xt * BN;
+  const int rows = (int)min((int64_t)BN, p.rows - row0);
+  // N results of this feature, `step` tokens apart from row0 + c0; residuals in flight together.
+  auto finish = [&](auto n, const float (&z)[decltype(n)::value], int c0, int step) {
+    constexpr int N = decltype(n)::value;
+    if (!in) return;
+    float r[N];
+    if (p.resid) {
+      const T* q = static_cast<const T*>(p.resid) + (row0 + c0) * p.ldr + col;
+      const int64_t d = p.ldr * step;
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[i] = c0 + i * step < rows ? to_f32(q[i * d]) : 0.f;
+    }
+    T* q = static_cast<T*>(p.y) + (row0 + c0) * p.ldy + col;
+    T* qp = static_cast<T*>(p.pre) + (row0 + c0) * p.ldp + col;
+    const int64_t d = p.ldy * step, dp = p.ldp * step;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (c0 + i * step >= rows) break;
+      const float v = z[i] + bias;
+      if (p.pre) qp[i * dp] = from_f32<T>(v);
+      float o = act_value<ACT>(v);
+      if (p.resid) o += r[i];
+      q[i * d] = from_f32<T>(o);
+    }
+  };
   mbar_wait(acc_full, 0, abort_flag);        // the ring is idle after it
   __syncwarp();
   tc_fence_after();
-  const int quad = warp & 3;
-  const int f = quad * 32 + lane;            // feature within the tile
-  const int64_t col = (int64_t)ft * 128 + f;
-  const bool epi = warp >= 2;
-  const float bias = epi && p.bias && col < p.cols ? to_f32(static_cast<const T*>(p.bias)[col]) : 0.f;
-  auto finish = [&](float z, int64_t row) {
-    if (row >= p.rows || col >= p.cols) return;
-    z += bias;
-    if (p.pre) static_cast<T*>(p.pre)[row * p.ldp + col] = from_f32<T>(z);
-    float v = act_value<ACT>(z);
-    if (p.resid) v += to_f32(static_cast<const T*>(p.resid)[row * p.ldr + col]);
-    static_cast<T*>(p.y)[row * p.ldy + col] = from_f32<T>(v);
-  };
-  const int64_t row0 = (int64_t)xt * BN;
-  __syncthreads();
-  if (epi) {
-    constexpr int CH = BN < 32 ? BN : 32;
+  if (split > 1) {
+    __syncthreads();
+    cluster_sync();                          // every ring of the cluster is
+  }
+  const int per = BN / split;
+  if (epi && !*abort_flag) {
 #pragma unroll 1
-    for (int c0 = 0; c0 < BN; c0 += CH) {
-      uint32_t r[32];
-      tmem_ld_32x32b_x32(tmem + ((uint32_t)(quad * 32) << 16) + c0, r);   // BN = 16: the upper columns are idle
+    for (int c0 = group * CH; c0 < BN; c0 += 2 * CH) {
+      if (c0 >= rows) break;
+      uint32_t r[CH];
+      tmem_ld(tmem + ((uint32_t)(quad * 32) << 16) + c0, r);
       tmem_ld_wait();
-      if (*abort_flag) continue;
       if (split == 1) {
+        float z[CH];
 #pragma unroll
-        for (int c = 0; c < CH; ++c) finish(__uint_as_float(r[c]), row0 + c0 + c);
+        for (int c = 0; c < CH; ++c) z[c] = __uint_as_float(r[c]);
+        finish(std::integral_constant<int, CH>{}, z, c0, 1);
       } else {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) parts[(c0 + c) * 128 + f] = __uint_as_float(r[c]);
+        for (int c = 0; c < CH; ++c) {
+          const int t = c0 + c, owner = t / per;
+          st_cluster(mapa_shared(&parts[((rank * per) + t - owner * per) * 128 + f], owner), __uint_as_float(r[c]));
+        }
       }
     }
   }
   tc_fence_before();
+  __syncwarp();
   __syncthreads();
   if (split > 1) {
-    cluster_sync();
-    if (epi) {                               // this CTA's share of the tile's tokens, ranks in order
-      const int per = BN / split;
-#pragma unroll 2
-      for (int c = rank * per; c < (rank + 1) * per; ++c) {
-        if (row0 + c >= p.rows) break;
-        const uint32_t at = smem_u32(&parts[c * 128 + f]);
-        float s = 0.f;
-        float v[8];
+    cluster_sync();                          // all parts are here; nothing remote happens after it
+    if (epi && !*abort_flag) {               // this CTA's tokens, ranks in order, two at a time
+      for (int t = group * 2; t < per; t += 4) {
+        float z[2];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (k < split) {
-            uint32_t remote;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(k));
-            v[k] = ld_cluster(remote);
-          }
+        for (int i = 0; i < 2; ++i) {
+          z[i] = 0.f;
+          for (int k = 0; k < split; ++k)
+            if (t + i < per) z[i] += parts[(k * per + t + i) * 128 + f];
         }
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (k < split) s += v[k];
-        finish(s, row0 + c);
+        if (t + 1 < per) finish(std::integral_constant<int, 2>{}, z, rank * per + t, 1);
+        else finish(std::integral_constant<int, 1>{}, reinterpret_cast<const float(&)[1]>(z), rank * per + t, 1);
       }
     }
-    cluster_sync();                          // no CTA leaves while its parts are read
   }
   if (warp == 1) {
     tc_fence_after();
@@ -646,13 +685,16 @@ __global__ void __launch_bounds__(256) dz_kernel(const T* dy, int64_t ldy, const
 }
 
 // ------------------------------------------------------------------------ host
+constexpr int kDevices = 64;
 struct Dev {
-  int sms = 0;
+  int index = 0, sms = 0;
 };
 static int device(Dev& d) {
-  int dev = 0;
-  VDN_CUDA_TRY(cudaGetDevice(&dev));
-  VDN_CUDA_TRY(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev));
+  static int sms[kDevices] = {};
+  VDN_CUDA_TRY(cudaGetDevice(&d.index));
+  VDN_CHECK_ARG(d.index >= 0 && d.index < kDevices, "device index out of range");
+  if (!sms[d.index]) VDN_CUDA_TRY(cudaDeviceGetAttribute(&sms[d.index], cudaDevAttrMultiProcessorCount, d.index));
+  d.sms = sms[d.index];
   return VDN_OK;
 }
 
@@ -681,11 +723,15 @@ struct Operand {
   bool mn;                                   // MN-major: stored [depth, rows]
 };
 
-template <typename K>
-static int allow_smem(K* kernel, size_t bytes) {   // once per kernel and device would do; the call is cheap
-  VDN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  return VDN_OK;
-}
+// Raises a kernel's shared-memory limit, once per device.
+#define VDN_ALLOW_SMEM(kernel, bytes, dev)                                                                    \
+  do {                                                                                                        \
+    static bool set[kDevices] = {};                                                                           \
+    if (!set[dev]) {                                                                                          \
+      VDN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(bytes))); \
+      set[dev] = true;                                                                                        \
+    }                                                                                                         \
+  } while (0)
 
 template <typename T, bool A_MN, bool B_MN, int ACT>
 static int run_pair(const Operand& x, const Operand& f, int64_t depth, Params p, const Dev& d, cudaStream_t stream) {
@@ -709,7 +755,8 @@ static int run_pair(const Operand& x, const Operand& f, int64_t depth, Params p,
   p.m_tiles = (int)((p.rows + 255) / 256);
   p.n_tiles = (int)((p.cols + 255) / 256);
   auto* kernel = pair_kernel<T, A_MN, B_MN, ACT>;
-  if (int rc = allow_smem(kernel, PAIR_SMEM)) return rc;
+  p.bias_vec = aligned16(p.bias);
+  VDN_ALLOW_SMEM(kernel, PAIR_SMEM, d.index);
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles, pairs = d.sms / 2;
   kernel<<<(unsigned)(2 * (tiles < pairs ? tiles : pairs)), PAIR_THREADS, PAIR_SMEM, stream>>>(ma, mb, my, mp, mr, p);
   VDN_LAUNCH_CHECK("linear (pair)");
@@ -726,11 +773,12 @@ static int run_narrow(const Operand& x, const Operand& f, int64_t depth, Params 
   p.m_tiles = (int)((p.cols + 127) / 128);
   p.n_tiles = (int)((p.rows + BN - 1) / BN);
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
-  // Two CTAs fit an SM: split the depth until they are there, but not below four blocks a CTA.
+  // Two CTAs fit an SM: split the depth while that leaves a fifth of the places free (clusters
+  // of eight do not pack into every GPC: a second wave cost 6 us of 11) and each CTA four blocks.
   int split = 1;
-  while (split < 8 && tiles * split * 2 <= 2 * d.sms + d.sms / 2 && p.k_blocks >= 8 * split) split *= 2;
+  while (split < 8 && tiles * split * 2 * 5 <= 2 * d.sms * 4 && p.k_blocks >= 8 * split) split *= 2;
   auto* kernel = narrow_kernel<T, F_MN, X_MN, ACT, BN>;
-  if (int rc = allow_smem(kernel, narrow_smem<BN>())) return rc;
+  VDN_ALLOW_SMEM(kernel, narrow_smem<BN>(), d.index);
   VDN_CHECK_ARG(tiles * split < (1ll << 31), "too many tiles for one launch");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * split));
@@ -754,9 +802,10 @@ static int product(const Operand& x, const Operand& f, int64_t depth, Params p, 
   if (int rc = device(d)) return rc;
   p.k_blocks = (int)((depth + BK - 1) / BK);
   const int64_t pair_tiles = ((p.rows + 255) / 256) * ((p.cols + 255) / 256);
-  // Fewer than 28 pair tiles leave most SMs without work; narrow tiles with a split depth fill them.
+  // Up to 128 rows would leave half of every pair tile empty, and fewer than 28 pair tiles most
+  // SMs without work; narrow tiles with a split depth fill them.
   VDN_CHECK_ARG(pair_tiles < (1ll << 29), "too many tiles for one launch");
-  if (pair_tiles >= 28) return run_pair<T, X_MN, F_MN, ACT>(x, f, depth, p, d, stream);
+  if (pair_tiles >= 28 && p.rows > 128) return run_pair<T, X_MN, F_MN, ACT>(x, f, depth, p, d, stream);
   if constexpr (!X_MN) {
     if (p.rows <= 16) return run_narrow<T, F_MN, X_MN, ACT, 16>(x, f, depth, p, d, stream);
     if (p.rows <= 32) return run_narrow<T, F_MN, X_MN, ACT, 32>(x, f, depth, p, d, stream);

@@ -22,13 +22,14 @@ _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def _rows(t):
-    """t as [rows, width] with unit column stride: a view where the layout allows it."""
-    flat = t.reshape(-1, t.shape[-1])
-    return flat if flat.stride(1) == 1 or flat.shape[1] == 1 else flat.contiguous()
-
-
-def _ld(flat):
-    return flat.stride(0) if flat.shape[0] > 1 else flat.shape[1]
+    """(t as rows of unit column stride, a view where the layout allows it; rows; row stride)"""
+    width = t.shape[-1]
+    if t.is_contiguous():
+        return t, t.numel() // width, width
+    flat = t.reshape(-1, width)
+    if flat.stride(1) != 1 and width != 1:
+        flat = flat.contiguous()
+    return flat, flat.shape[0], flat.stride(0) if flat.shape[0] > 1 else width
 
 
 def _check(x, weight, bias):
@@ -39,31 +40,36 @@ def _check(x, weight, bias):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("x must have a last dimension to normalise")
     _lib.require_device(x, "x")
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is None:
-            continue
-        if t.dtype not in (x.dtype, torch.float32):
-            raise TypeError(f"{name} must be {x.dtype} or fp32, got {t.dtype}")
-        if t.shape != (x.shape[-1],) or t.device != x.device:
-            raise ValueError(f"{name} must be [{x.shape[-1]}] on x's device")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise TypeError("weight and bias must share one dtype")
+    if weight is not None:
+        _check_parameter(x, weight, "weight")
+    if bias is not None:
+        _check_parameter(x, bias, "bias")
+        if weight is not None and weight.dtype != bias.dtype:
+            raise TypeError("weight and bias must share one dtype")
+
+
+def _check_parameter(x, t, name):
+    if t.dtype != x.dtype and t.dtype != torch.float32:
+        raise TypeError(f"{name} must be {x.dtype} or fp32, got {t.dtype}")
+    if t.dim() != 1 or t.shape[0] != x.shape[-1] or t.device != x.device:
+        raise ValueError(f"{name} must be [{x.shape[-1]}] on x's device")
 
 
 def _forward(x, weight, bias, eps, stats):
     _check(x, weight, bias)
-    flat = _rows(x)
-    rows, width = flat.shape
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    flat, rows, ld = _rows(x)
+    width = x.shape[-1]
+    device, code = x.device, _lib.dtype_code(x.dtype)
+    y = torch.empty(x.shape, dtype=x.dtype, device=device)
     mean = rstd = None
     if stats:
-        mean, rstd = torch.empty(2, rows, dtype=torch.float32, device=x.device)
+        mean, rstd = torch.empty(2, rows, dtype=torch.float32, device=device)
     given = weight if weight is not None else bias
     w = None if weight is None else weight.contiguous()
     b = None if bias is None else bias.contiguous()
-    _lib.call_on(x.device, "vdn_layer_norm", flat.data_ptr(), _lib.dtype_code(x.dtype), rows, width, _ld(flat),
-                 _lib.ptr(w), _lib.ptr(b), _lib.dtype_code(x.dtype if given is None else given.dtype), float(eps),
-                 y.data_ptr(), width, _lib.ptr(mean), _lib.ptr(rstd))
+    _lib.call_on(device, "vdn_layer_norm", flat.data_ptr(), code, rows, width, ld, _lib.address(w), _lib.address(b),
+                 code if given is None else _lib.dtype_code(given.dtype), eps, y.data_ptr(), width,
+                 _lib.address(mean), _lib.address(rstd))
     return y, mean, rstd
 
 
@@ -86,7 +92,7 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x, weight=None, bias=None, eps=1e-5, *, return_stats=False):
     """y of x's shape and dtype; with return_stats also the rows' mean and 1 / sqrt(var + eps)
     (fp32 [rows], what layer_norm_backward takes)."""
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, bias)):
+    if torch.is_grad_enabled() and _lib.records(x, weight, bias):
         if return_stats:
             raise ValueError("return_stats is for the explicit backward, not where gradients are recorded")
         _lib.refuse_captured_autograd("layer_norm")
@@ -99,8 +105,8 @@ def _backward(grad_y, x, weight, mean, rstd, want_w, want_b, bias_dtype=None):
     _check(x, weight, None)
     if grad_y.shape != x.shape or grad_y.dtype != x.dtype or grad_y.device != x.device:
         raise ValueError("grad_y must match x in shape, dtype and device")
-    flat, dy = _rows(x), _rows(grad_y)
-    rows, width = flat.shape
+    (flat, rows, x_ld), (dy, _, dy_ld) = _rows(x), _rows(grad_y)
+    width = x.shape[-1]
     for t, name in ((mean, "mean"), (rstd, "rstd")):
         if t.shape != (rows,) or t.dtype != torch.float32 or t.device != x.device:
             raise ValueError(f"{name} must be fp32 [{rows}] on x's device")
@@ -112,9 +118,9 @@ def _backward(grad_y, x, weight, mean, rstd, want_w, want_b, bias_dtype=None):
     ws = torch.empty(need, dtype=torch.uint8, device=x.device)
     w = None if weight is None else weight.contiguous()
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    _lib.call_on(x.device, "vdn_layer_norm_backward", dy.data_ptr(), _lib.dtype_code(x.dtype), rows, width, _ld(dy),
-                 flat.data_ptr(), _ld(flat), _lib.ptr(w), _lib.dtype_code(kind), mean.data_ptr(), rstd.data_ptr(),
-                 dx.data_ptr(), width, _lib.ptr(dw), _lib.ptr(db), ws.data_ptr(), need)
+    _lib.call_on(x.device, "vdn_layer_norm_backward", dy.data_ptr(), _lib.dtype_code(x.dtype), rows, width, dy_ld,
+                 flat.data_ptr(), x_ld, _lib.address(w), _lib.dtype_code(kind), mean.data_ptr(), rstd.data_ptr(),
+                 dx.data_ptr(), width, _lib.address(dw), _lib.address(db), ws.data_ptr(), need)
     return dx, dw, db
 
 

@@ -28,30 +28,39 @@ def _pad8(n):
     return (n + 7) // 8 * 8
 
 
-def _operand(t):
-    """t [rows, cols] as the tensor maps take it: unit column stride, 16-byte aligned rows
-    (copied into padded rows where its layout does not suit them)."""
-    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
-        return t
-    return torch.empty(t.shape[0], _pad8(t.shape[1]), dtype=t.dtype, device=t.device)[:, :t.shape[1]].copy_(t)
+def _operand(t, cols):
+    """t [..., cols] as the tensor maps take it: (rows of unit column stride, each 16-byte
+    aligned; their count; their stride), copied into padded rows where its layout does not suit them."""
+    if t.is_contiguous() and cols % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t, t.numel() // cols, cols
+    flat = t.reshape(-1, cols)
+    ld = flat.stride(0)
+    if flat.stride(1) != 1 or ld % 8 or ld < cols or flat.data_ptr() % 16:
+        ld = _pad8(cols)
+        flat = torch.empty(flat.shape[0], ld, dtype=t.dtype, device=t.device)[:, :cols].copy_(flat)
+    return flat, flat.shape[0], ld
 
 
 def _matrix(t, cols):
-    """t [..., cols] as [rows, cols] with unit column stride (any row stride)."""
+    """t [..., cols] as (rows of unit column stride, their count, their stride)."""
+    if t.is_contiguous():
+        return t, t.numel() // cols, cols
     flat = t.reshape(-1, cols)
-    return flat if flat.stride(1) == 1 or cols == 1 else flat.contiguous()
+    if flat.stride(1) != 1 and cols != 1:
+        flat = flat.contiguous()
+    return flat, flat.shape[0], flat.stride(0)
 
 
 def _check(x, weight, act):
     if not isinstance(x, torch.Tensor) or not isinstance(weight, torch.Tensor):
         raise TypeError("x and weight must be tensors")
-    if x.dtype not in (torch.bfloat16, torch.float16) or weight.dtype != x.dtype:
+    if (x.dtype != torch.bfloat16 and x.dtype != torch.float16) or weight.dtype != x.dtype:
         raise TypeError(f"x and weight must both be bf16 or both fp16, got {x.dtype} and {weight.dtype}")
     if not x.is_cuda or weight.device != x.device:
         raise ValueError("x and weight must be CUDA tensors on one device")
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError("x must be [..., k] and weight [n, k]")
-    if weight.shape[0] < 1 or weight.shape[1] < 1:
+    if weight.numel() < 1:
         raise ValueError("weight must not be empty")
     if act not in ACTIVATIONS:
         raise ValueError(f"act must be one of {tuple(ACTIVATIONS)}, got {act!r}")
@@ -69,20 +78,23 @@ def _forward(x, weight, bias, act, residual, want_pre):
     _check(x, weight, act)
     n, k = weight.shape
     shape = (*x.shape[:-1], n)
+    device = x.device
+    res = pre = None
+    ldr = 0
     if bias is not None:
         _same(bias, x, (n,), "bias")
         bias = bias.contiguous()
     if residual is not None:
         _same(residual, x, shape, "residual")
-    flat = _operand(x.reshape(-1, k))
-    w = _operand(weight)
-    rows = flat.shape[0]
-    res = None if residual is None else _matrix(residual, n)
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    pre = torch.empty(shape, dtype=x.dtype, device=x.device) if want_pre else None
-    _lib.call_on(x.device, "vdn_linear_act", flat.data_ptr(), flat.stride(0), w.data_ptr(), w.stride(0),
-                 _lib.ptr(bias), _lib.ptr(res), res.stride(0) if res is not None else 0, _lib.dtype_code(x.dtype),
-                 ACTIVATIONS[act], rows, n, k, y.data_ptr(), n, _lib.ptr(pre), n, _status(x.device).data_ptr())
+        res, _, ldr = _matrix(residual, n)
+    flat, rows, ldx = _operand(x, k)
+    w, _, ldw = _operand(weight, k)
+    y = torch.empty(shape, dtype=x.dtype, device=device)
+    if want_pre:
+        pre = torch.empty(shape, dtype=x.dtype, device=device)
+    _lib.call_on(device, "vdn_linear_act", flat.data_ptr(), ldx, w.data_ptr(), ldw, _lib.address(bias),
+                 _lib.address(res), ldr, _lib.dtype_code(x.dtype), ACTIVATIONS[act], rows, n, k, y.data_ptr(), n,
+                 _lib.address(pre), n, _status(device).data_ptr())
     return y, pre
 
 
@@ -110,8 +122,7 @@ def linear_act(x, weight, bias=None, *, act="none", residual=None, return_pre=Fa
 
     Row-strided operands are read in place where their rows are 16-byte aligned, others
     (odd k, transposed) are copied into padded rows first."""
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
-                                       for t in (x, weight, bias, residual)):
+    if torch.is_grad_enabled() and _lib.records(x, weight, bias, residual):
         if return_pre:
             raise ValueError("return_pre is for the explicit backward, not where gradients are recorded")
         _lib.refuse_captured_autograd("linear_act")
@@ -130,31 +141,34 @@ def _backward(grad_y, x, weight, pre, act, want_x, want_w, want_b):
             raise ValueError("pre (linear_act's return_pre) is needed for the activation's gradient")
         _same(pre, x, shape, "pre")
     dev, code, word = x.device, _lib.dtype_code(x.dtype), _status(x.device).data_ptr()
-    dy = _matrix(grad_y, n)
-    rows = dy.shape[0]
-    db = torch.empty(n, dtype=x.dtype, device=dev) if want_b else None
-    need = _lib.load().vdn_linear_dz_workspace_size(rows, n) if want_b else 0
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if want_b else None
-    dz, z = dy, None
+    dz, rows, ldz = _matrix(grad_y, n)
+    db = ws = z = None
+    need = ldp = 0
+    if want_b:
+        db = torch.empty(n, dtype=x.dtype, device=dev)
+        need = _lib.load().vdn_linear_dz_workspace_size(rows, n)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    dy, ldy = dz, ldz
     if act != "none":
-        z = _matrix(pre, n)
-        dz = torch.empty(rows, _pad8(n), dtype=x.dtype, device=dev)[:, :n]
+        z, _, ldp = _matrix(pre, n)
+        ldz = _pad8(n)
+        dz = torch.empty(rows, ldz, dtype=x.dtype, device=dev)[:, :n]
     if want_b or act != "none":
-        _lib.call_on(dev, "vdn_linear_dz", dy.data_ptr(), dy.stride(0), _lib.ptr(z), z.stride(0) if z is not None else 0,
-                     code, ACTIVATIONS[act], rows, n, dz.data_ptr(), dz.stride(0), _lib.ptr(db), _lib.ptr(ws), need)
+        _lib.call_on(dev, "vdn_linear_dz", dy.data_ptr(), ldy, _lib.address(z), ldp, code, ACTIVATIONS[act], rows, n,
+                     dz.data_ptr(), ldz, _lib.address(db), _lib.address(ws), need)
     dx = dw = None
     if want_x or want_w:
-        dz = _operand(dz)
+        dz, _, ldz = _operand(dz, n)
     if want_x:
-        w = _operand(weight)
+        w, _, ldw = _operand(weight, k)
         dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        _lib.call_on(dev, "vdn_linear_dx", dz.data_ptr(), dz.stride(0), w.data_ptr(), w.stride(0), code, rows, n, k,
-                     dx.data_ptr(), k, word)
+        _lib.call_on(dev, "vdn_linear_dx", dz.data_ptr(), ldz, w.data_ptr(), ldw, code, rows, n, k, dx.data_ptr(), k,
+                     word)
     if want_w:
-        flat = _operand(x.reshape(-1, k))
+        flat, _, ldx = _operand(x, k)
         dw = torch.empty(n, k, dtype=x.dtype, device=dev)
-        _lib.call_on(dev, "vdn_linear_dw", dz.data_ptr(), dz.stride(0), flat.data_ptr(), flat.stride(0), code, rows, n,
-                     k, dw.data_ptr(), k, word)
+        _lib.call_on(dev, "vdn_linear_dw", dz.data_ptr(), ldz, flat.data_ptr(), ldx, code, rows, n, k, dw.data_ptr(),
+                     k, word)
     return dx, dw, db
 
 

@@ -29,89 +29,91 @@ def _layout(x, log_decay, state, cu_seqlens, what):
         raise TypeError(f"{what} and log_decay must be tensors")
     if x.dtype not in _DTYPES:
         raise TypeError(f"{what} must be fp32, bf16 or fp16, got {x.dtype}")
-    if log_decay.dtype not in (x.dtype, torch.float32):
+    if log_decay.dtype != x.dtype and log_decay.dtype != torch.float32:
         raise TypeError(f"log_decay must be {x.dtype} or fp32, got {log_decay.dtype}")
     if not x.is_cuda or log_decay.device != x.device:
         raise ValueError(f"{what} and log_decay must be CUDA tensors on one device")
     _lib.require_device(x, what)
     lead = 2 if cu_seqlens is None else 1
-    if x.dim() - lead not in (1, 2):
+    shape = x.shape
+    dims = len(shape) - lead
+    if dims == 2:
+        heads, d = shape[-2:]
+    elif dims == 1:
+        heads, d = 1, shape[-1]
+    else:
         raise ValueError(f"{what} must be [B, T, C] or [B, T, H, d] (packed: [N, C] or [N, H, d])")
-    tail = x.shape[lead:]
-    heads, d = (tail[0], tail[1]) if len(tail) == 2 else (1, tail[0])
-    shared = log_decay.dim() == lead + 1 and len(tail) == 2
-    if log_decay.shape != (x.shape[:-1] if shared else x.shape):
+    shared = dims == 2 and log_decay.dim() == lead + 1
+    if log_decay.shape != (shape[:-1] if shared else shape):
         raise ValueError(f"log_decay must have {what}'s shape, or one value per head of [.., H, d]")
     if shared and d not in (32, 64, 128):
         raise ValueError("a decay per head needs a head dim of 32, 64 or 128 (expand it per channel for others)")
     if cu_seqlens is None:
-        seqs, rows = x.shape[:2]
+        seqs, rows = shape[0], shape[1]
     else:
         if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.device != x.device:
             raise ValueError("cu_seqlens must be int32 [sequences + 1] on the device of the rows")
         if cu_seqlens.numel() < 1 or not cu_seqlens.is_contiguous():
             raise ValueError("cu_seqlens must be contiguous and hold at least one offset")
-        seqs, rows = cu_seqlens.numel() - 1, x.shape[0]
-    _check_state(state, x, (seqs, *tail), "state")
+        seqs, rows = cu_seqlens.numel() - 1, shape[0]
+    if state is not None:
+        _check_state(state, x, (seqs, *shape[lead:]), "state")
     return lead, seqs, rows, heads, d, shared
 
 
 def _check_state(state, x, shape, name):
-    if state is None:
-        return
     if state.dtype != torch.float32 or state.device != x.device:
         raise TypeError(f"{name} must be fp32 on the device of the rows")
     if state.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(state.shape)}")
 
 
-def _flat(t, lead):
-    """t with its trailing dims laid out as one contiguous row of channels (copied if not)."""
-    size, stride = t.shape[lead:], t.stride()[lead:]
-    need = 1
-    for n, s in zip(reversed(size), reversed(stride)):
-        if n != 1 and s != need:
-            return t.contiguous()
-        need *= n
-    return t
-
-
-def _strides(t, lead):
-    """(batch stride, row stride); a stride that no index multiplies counts as 0."""
-    row = t.stride(lead - 1) if t.shape[lead - 1] > 1 else 0
-    return (t.stride(0) if t.shape[0] > 1 else 0) if lead == 2 else 0, row
-
-
-def _output(out, x, lead, name):
-    if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
-        raise ValueError(f"{name} must match the rows in shape, dtype and device")
-    if _flat(out, lead) is not out:
-        raise ValueError(f"{name}'s channels must be contiguous")
-    return out
+def _rows(t, lead, channels):
+    """(t with each row's channels contiguous, copied if they are not; batch stride; row
+    stride).  A stride that no index multiplies counts as 0."""
+    shape = t.shape
+    if not t.is_contiguous():
+        need = 1
+        for n, s in zip(reversed(shape[lead:]), reversed(t.stride()[lead:])):
+            if n != 1 and s != need:
+                t = t.contiguous()
+                break
+            need *= n
+        stride = t.stride()
+        row = stride[lead - 1] if shape[lead - 1] > 1 else 0
+        return t, (stride[0] if shape[0] > 1 else 0) if lead == 2 else 0, row
+    if lead == 1:
+        return t, 0, channels if shape[0] > 1 else 0
+    return t, channels * shape[1] if shape[0] > 1 else 0, channels if shape[1] > 1 else 0
 
 
 def _forward(x, log_decay, state, cu_seqlens, reverse, out, out_state):
     lead, seqs, rows, heads, d, shared = _layout(x, log_decay, state, cu_seqlens, "x")
-    y = _output(out, x, lead, "out")
-    shape = (seqs, *x.shape[lead:])
+    shape, device, channels = (seqs, *x.shape[lead:]), x.device, heads * d
+    y = torch.empty(x.shape, dtype=x.dtype, device=device) if out is None else out
+    if out is not None:
+        if out.shape != x.shape or out.dtype != x.dtype or out.device != device:
+            raise ValueError("out must match x in shape, dtype and device")
+        if _rows(out, lead, channels)[0] is not out:
+            raise ValueError("out's channels must be contiguous")
     if out_state is None:
-        out_state = torch.empty(shape, dtype=torch.float32, device=x.device)
+        out_state = torch.empty(shape, dtype=torch.float32, device=device)
     else:
         _check_state(out_state, x, shape, "out_state")
         if not out_state.is_contiguous():
             raise ValueError("out_state must be contiguous")
-    if heads * d == 0:
+    if channels == 0:
         return y, out_state
     if seqs == 0:
         return (y.zero_() if out is None else y), out_state
-    x, log_decay = _flat(x, lead), _flat(log_decay, lead)
+    x, x_batch, x_row = _rows(x, lead, channels)
+    log_decay, g_batch, g_row = _rows(log_decay, lead, heads if shared else channels)
+    _, y_batch, y_row = _rows(y, lead, channels)
     state = None if state is None else state.contiguous()
-    _lib.call_on(x.device, "vdn_gated_scan", x.data_ptr(), _lib.dtype_code(x.dtype), *_strides(x, lead),
-                 log_decay.data_ptr(), _lib.dtype_code(log_decay.dtype), *_strides(log_decay, lead), int(shared),
-                 _lib.ptr(state), _lib.ptr(cu_seqlens), seqs, rows, heads, d, int(bool(reverse)), y.data_ptr(),
-                 *_strides(y, lead), int(out is None), out_state.data_ptr(), _status(x.device).data_ptr())
+    _lib.call_on(device, "vdn_gated_scan", x.data_ptr(), _lib.dtype_code(x.dtype), x_batch, x_row,
+                 log_decay.data_ptr(), _lib.dtype_code(log_decay.dtype), g_batch, g_row, shared, _lib.address(state),
+                 _lib.address(cu_seqlens), seqs, rows, heads, d, reverse, y.data_ptr(), y_batch, y_row, out is None,
+                 out_state.data_ptr(), _status(device).data_ptr())
     return y, out_state
 
 
@@ -147,13 +149,12 @@ def gated_scan(x, log_decay, state=None, *, cu_seqlens=None, reverse=False, out=
     its last row to its first.  Strided rows and expanded log_decay are read in place as
     long as a row's channels are contiguous.  A state that overflows fp32 comes out as inf or NaN.
     """
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
-                                       for t in (x, log_decay, state)):
+    if torch.is_grad_enabled() and _lib.records(x, log_decay, state):
         if out is not None or out_state is not None:
             raise ValueError("out and out_state cannot be given where gradients are recorded")
         _lib.refuse_captured_autograd("gated_scan")
         return _GatedScan.apply(x, log_decay, state, cu_seqlens, bool(reverse))
-    return _forward(x, log_decay, state, cu_seqlens, reverse, out, out_state)
+    return _forward(x, log_decay, state, cu_seqlens, bool(reverse), out, out_state)
 
 
 @torch.no_grad()
@@ -167,19 +168,25 @@ def gated_scan_backward(grad_y, log_decay, y, *, state=None, grad_state=None, cu
     if grad_y.shape != y.shape or grad_y.dtype != y.dtype or grad_y.device != y.device:
         raise ValueError("grad_y must match y in shape, dtype and device")
     shape = (seqs, *y.shape[lead:])
-    _check_state(grad_state, y, shape, "grad_state")
-    dx = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-    dg = torch.empty(log_decay.shape, dtype=log_decay.dtype, device=y.device)
-    ds = torch.empty(shape, dtype=torch.float32, device=y.device)
-    if heads * d == 0 or seqs == 0:
+    if grad_state is not None:
+        _check_state(grad_state, y, shape, "grad_state")
+        grad_state = grad_state.contiguous()
+    device, channels = y.device, heads * d
+    dx = torch.empty(y.shape, dtype=y.dtype, device=device)
+    dg = torch.empty(log_decay.shape, dtype=log_decay.dtype, device=device)
+    ds = torch.empty(shape, dtype=torch.float32, device=device)
+    if channels == 0 or seqs == 0:
         return dx.zero_(), dg.zero_(), ds
-    grad_y, log_decay, y = _flat(grad_y, lead), _flat(log_decay, lead), _flat(y, lead)
+    decays = heads if shared else channels
+    grad_y, dy_batch, dy_row = _rows(grad_y, lead, channels)
+    log_decay, g_batch, g_row = _rows(log_decay, lead, decays)
+    y, y_batch, y_row = _rows(y, lead, channels)
+    _, dx_batch, dx_row = _rows(dx, lead, channels)
+    _, dg_batch, dg_row = _rows(dg, lead, decays)
     state = None if state is None else state.contiguous()
-    grad_state = None if grad_state is None else grad_state.contiguous()
-    _lib.call_on(y.device, "vdn_gated_scan_backward", grad_y.data_ptr(), _lib.dtype_code(y.dtype),
-                 *_strides(grad_y, lead), log_decay.data_ptr(), _lib.dtype_code(log_decay.dtype),
-                 *_strides(log_decay, lead), int(shared), y.data_ptr(), *_strides(y, lead), _lib.ptr(state),
-                 _lib.ptr(grad_state), _lib.ptr(cu_seqlens), seqs, rows, heads, d, int(bool(reverse)),
-                 dx.data_ptr(), *_strides(dx, lead), dg.data_ptr(), *_strides(dg, lead), 1, ds.data_ptr(),
-                 _status(y.device).data_ptr())
+    _lib.call_on(device, "vdn_gated_scan_backward", grad_y.data_ptr(), _lib.dtype_code(y.dtype), dy_batch, dy_row,
+                 log_decay.data_ptr(), _lib.dtype_code(log_decay.dtype), g_batch, g_row, shared, y.data_ptr(), y_batch,
+                 y_row, _lib.address(state), _lib.address(grad_state), _lib.address(cu_seqlens), seqs, rows, heads, d,
+                 bool(reverse), dx.data_ptr(), dx_batch, dx_row, dg.data_ptr(), dg_batch, dg_row, True,
+                 ds.data_ptr(), _status(device).data_ptr())
     return dx, dg, ds
