@@ -431,13 +431,14 @@ int vdn_layer_norm(const void* x, int dtype, int64_t rows, int64_t width, int64_
                    int64_t y_stride, float* mean, float* rstd, cudaStream_t stream);
 
 /* Gradients of vdn_layer_norm: dx (dtype), d_weight and d_bias (w_dtype, either may be
- * NULL), the two summed over the rows in fp32 and in a fixed order through the workspace. */
+ * NULL), the two summed over the rows in fp32 and in a fixed order through the workspace.
+ * status: as in vdn_mxfp8_gemm. */
 size_t vdn_layer_norm_backward_workspace_size(int64_t rows, int64_t width);
 int vdn_layer_norm_backward(const void* dy, int dtype, int64_t rows, int64_t width, int64_t dy_stride,
                             const void* x, int64_t x_stride, const void* weight, int w_dtype,
                             const float* mean, const float* rstd, void* dx, int64_t dx_stride,
                             void* d_weight, void* d_bias, void* workspace, size_t workspace_bytes,
-                            cudaStream_t stream);
+                            int* status, cudaStream_t stream);
 
 /* Linear layer on tcgen05, 16-bit operands (`dtype` bf16 or fp16, all matrices alike), fp32
  * accumulation: z = x w^T + bias, pre = z (if not NULL), y = act(z) + residual (if not

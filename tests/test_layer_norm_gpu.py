@@ -61,7 +61,7 @@ def _check(cuda, x, w, b, dy, eps=1e-5):
     got = grads[0].double().cpu()
     assert grads[0].dtype == x.dtype
     assert bool(((got - dx).abs() <= err + _half(x.dtype) * (dx.abs() + err) + tiny).all())
-    chain = rows / 296 + 64 + 48      # rows of one CTA, lane groups, lines
+    chain = rows / 296 + 16 + 2960 / 32 + 32      # rows of one CTA, its lane groups, at most 2960 lines in 32 groups
     for got, want, mag, extra, on in ((grads[1], (d * xh).sum(0), (d * xh).abs().sum(0), (d.abs() * e_xh).sum(0), w is not None),
                                       (grads[2], d.sum(0), d.abs().sum(0), 0.0, b is not None)):
         if not on:

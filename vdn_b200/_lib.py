@@ -82,7 +82,7 @@ SIGNATURES = {
     "vdn_layer_norm": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _p, _i32, _f32, _p, _i64, _p, _p, _p]),
     "vdn_layer_norm_backward_workspace_size": (_sz, [_i64, _i64]),
     "vdn_layer_norm_backward": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _i32, _p, _p, _p, _i64, _p, _p,
-                                       _p, _sz, _p]),
+                                       _p, _sz, _p, _p]),
     "vdn_linear_act": (_i32, [_p, _i64, _p, _i64, _p, _p, _i64, _i32, _i32, _i64, _i64, _i64, _p, _i64, _p, _i64,
                               _p, _p]),
     "vdn_linear_dz_workspace_size": (_sz, [_i64, _i64]),

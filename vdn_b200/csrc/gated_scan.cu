@@ -59,18 +59,6 @@ struct Params {
   int* status;
 };
 
-// One channel (float) or two (f2, packed fp32 pairs) at a time.
-__device__ __forceinline__ float vset(float, float c) { return c; }
-__device__ __forceinline__ f2 vset(f2, float c) { return f2_pack(c, c); }
-__device__ __forceinline__ float vadd(float a, float b) { return a + b; }
-__device__ __forceinline__ f2 vadd(f2 a, f2 b) { return f2_add(a, b); }
-__device__ __forceinline__ float vmul(float a, float b) { return a * b; }
-__device__ __forceinline__ f2 vmul(f2 a, f2 b) { return f2_mul(a, b); }
-__device__ __forceinline__ float vfma(float a, float b, float c) { return fmaf(a, b, c); }
-__device__ __forceinline__ f2 vfma(f2 a, f2 b, f2 c) { return f2_fma(a, b, c); }
-template <int VEC> struct Lanes { using V = f2; static constexpr int N = VEC / 2; };
-template <> struct Lanes<1> { using V = float; static constexpr int N = 1; };
-
 // 2^n from the low bits of t = fp32(n + 127 + 1.5 * 2^23); 0 for n = -127, inf for n = 128.
 __device__ __forceinline__ float two_to(float t) { return __uint_as_float(__float_as_uint(t) << 23); }
 __device__ __forceinline__ f2 two_to(f2 t) {
@@ -112,33 +100,6 @@ __device__ __forceinline__ V decay_of(V g) {
   V hi, lo;
   decay_pair(g, hi, lo);
   return vadd(hi, lo);
-}
-
-__device__ __forceinline__ void spread(float a, float& v) { v = a; }
-__device__ __forceinline__ void spread(float a, f2& v) { v = f2_pack(a, a); }
-__device__ __forceinline__ void spread(f2 a, f2& v) { v = a; }
-
-__device__ __forceinline__ void to_lanes(const float (&e)[1], float (&v)[1]) { v[0] = e[0]; }
-template <int VEC> __device__ __forceinline__ void to_lanes(const float (&e)[VEC], f2 (&v)[VEC / 2]) {
-#pragma unroll
-  for (int i = 0; i < VEC / 2; ++i) v[i] = f2_pack(e[2 * i], e[2 * i + 1]);
-}
-__device__ __forceinline__ void from_lanes(const float (&v)[1], float (&e)[1]) { e[0] = v[0]; }
-template <int VEC> __device__ __forceinline__ void from_lanes(const f2 (&v)[VEC / 2], float (&e)[VEC]) {
-#pragma unroll
-  for (int i = 0; i < VEC / 2; ++i) f2_unpack(v[i], e[2 * i], e[2 * i + 1]);
-}
-template <typename T, int VEC, typename V, int N>
-__device__ __forceinline__ void unpack_lanes(const Raw<T, VEC>& raw, V (&v)[N]) {
-  float e[VEC];
-  unpack<T, VEC>(raw, e);
-  to_lanes(e, v);
-}
-template <typename T, int VEC, typename V, int N>
-__device__ __forceinline__ Raw<T, VEC> pack_lanes(const V (&v)[N]) {
-  float e[VEC];
-  from_lanes(v, e);
-  return pack<T, VEC>(e);
 }
 
 // A run's map c -> a c + h.

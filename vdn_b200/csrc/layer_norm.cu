@@ -15,7 +15,10 @@
 // them; one line of partial sums per CTA goes to the caller's workspace, and a second
 // kernel adds the lines in a fixed order.  No atomics: the same bits on every run.
 // Widths that fit no register form take `wide` kernels, which read a row again for each pass.
+#include <initializer_list>
+
 #include "train_common.cuh"
+#include "sm100.cuh"
 
 namespace vdn {
 namespace lnorm {
@@ -40,95 +43,261 @@ struct Bwd {
   float* part;          // [gridDim.x, 2, width]
   int64_t rows, dy_ld, x_ld, dx_ld;
   int width;
+  int* status;
 };
 
-// Sum over the `lanes` threads of a row: a lane group, or the whole block (0).
-template <int LANES>
-__device__ __forceinline__ float row_sum(float v, float* scratch) {
-  if constexpr (LANES > 0) {
+// The sums of N values over a row's threads: a lane group, or the whole block (LANES = 0: one
+// barrier; callers alternate between two `scratch` areas, so none is needed after the reads).
+template <int LANES, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float (*scratch)[32]) {
 #pragma unroll
-    for (int o = LANES / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-  } else {
+  for (int o = (LANES ? LANES : 32) / 2; o; o >>= 1)
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    const int warps = blockDim.x >> 5;
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  if constexpr (LANES == 0) {
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    if (lane < N) {
+      float mine = v[0];
+#pragma unroll
+      for (int i = 1; i < N; ++i) mine = lane == i ? v[i] : mine;
+      scratch[lane][threadIdx.x >> 5] = mine;
+    }
     __syncthreads();
-    v = 0.f;
-    for (int w = 0; w < warps; ++w) v += scratch[w];
-    return v;             // the caller alternates scratch halves, so no barrier after the reads
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = lane < warps ? scratch[i][lane] : 0.f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
   }
 }
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v, float (*scratch)[32]) {
+  float one[1] = {v};
+  row_sums<LANES>(one, scratch);
+  return one[0];
+}
+__device__ __forceinline__ float hsum(float v) { return v; }
+__device__ __forceinline__ float hsum(f2 v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return a + b;
+}
 
+// VEC weights (or biases) as they lie in memory, in 16-byte pieces or one smaller one.
 template <typename TW, int VEC>
-__device__ __forceinline__ void load_weight(const void* w, int col, float fill, float (&v)[VEC]) {
-  if (!w) {
+struct Weights {
+  static constexpr int STEP = sizeof(TW) * VEC > 16 ? 16 / (int)sizeof(TW) : VEC, N = VEC / STEP;
+  Raw<TW, STEP> raw[N];
+  __device__ __forceinline__ void load(const void* w, int col) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = fill;
-    return;
+    for (int i = 0; i < N; ++i) raw[i] = *reinterpret_cast<const Raw<TW, STEP>*>(static_cast<const TW*>(w) + col + i * STEP);
   }
-  constexpr int STEP = sizeof(TW) * VEC > 16 ? 16 / sizeof(TW) : VEC;
-#pragma unroll
-  for (int i = 0; i < VEC; i += STEP) {
-    float part[STEP];
-    unpack<TW, STEP>(*reinterpret_cast<const Raw<TW, STEP>*>(static_cast<const TW*>(w) + col + i), part);
-#pragma unroll
-    for (int j = 0; j < STEP; ++j) v[i + j] = part[j];
+  template <typename V, int M>
+  __device__ __forceinline__ void get(V (&v)[M]) const {
+    float e[VEC];
+    values(e);
+    to_lanes(e, v);
   }
-}
-
-template <typename T, typename TW, int VEC, int NV, int LANES, int MAXT>
-__global__ void __launch_bounds__(MAXT) forward_kernel(const Fwd p) {
-  using R = Raw<T, VEC>;
-  __shared__ float scratch[2][32];
-  const int lanes = LANES ? LANES : blockDim.x;
-  const int t = LANES ? threadIdx.x % (LANES ? LANES : 1) : threadIdx.x;
-  const int64_t row = LANES ? (int64_t)blockIdx.x * (blockDim.x / lanes) + threadIdx.x / lanes : blockIdx.x;
-  const bool on = row < p.rows;                      // uniform over the row's lanes
-  const T* x = static_cast<const T*>(p.x) + (on ? row : 0) * p.x_ld;
-  R raw[NV];
+  __device__ __forceinline__ void values(float (&v)[VEC]) const {
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int col = (t + k * lanes) * VEC;
-    raw[k] = on && col < p.width ? load_once<R>(x + col) : raw_zero<R>();
-  }
-  float v[NV][VEC], sum = 0.f;
+    for (int i = 0; i < N; ++i) {
+      float part[STEP];
+      unpack<TW, STEP>(raw[i], part);
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    unpack<T, VEC>(raw[k], v[k]);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) sum += v[k][i];
-  }
-  const float inv = 1.0f / (float)p.width;
-  const float mean = row_sum<LANES>(sum, scratch[0]) * inv;
-  float sq = 0.f;
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const bool in = (t + k * lanes) * VEC < p.width;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      v[k][i] -= mean;
-      if (in) sq = fmaf(v[k][i], v[k][i], sq);
+      for (int j = 0; j < STEP; ++j) v[i * STEP + j] = part[j];
     }
   }
-  const float rstd = rsqrtf(row_sum<LANES>(sq, scratch[1]) * inv + p.eps);
-  if (!on) return;
-  if (t == 0) {
-    if (p.mean) p.mean[row] = mean;
-    if (p.rstd) p.rstd[row] = rstd;
+};
+
+// Each CTA walks rows (blockIdx.x, + gridDim.x, ..) with the next row's loads in flight and the
+// weights of its columns in registers (HELD; else read again for every row, from L1).
+template <typename T, typename TW, int VEC, int NV, int LANES, int MAXT, int PER_SM, bool HELD>
+__global__ void __launch_bounds__(MAXT, PER_SM) forward_kernel(const Fwd p) {
+  using R = Raw<T, VEC>;
+  __shared__ float scratch[2][2][32];
+  const int lanes = LANES ? LANES : blockDim.x;
+  const int t = LANES ? threadIdx.x % (LANES ? LANES : 1) : threadIdx.x;
+  const int groups = LANES ? blockDim.x / lanes : 1;       // rows a CTA walks side by side
+  const int64_t stride = (int64_t)gridDim.x * groups;
+  const float inv = 1.0f / (float)p.width;
+  Weights<TW, VEC> w[HELD ? NV : 1], b[HELD ? NV : 1];
+  if constexpr (HELD) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int col = (t + k * lanes) * VEC;
+      if (col >= p.width) continue;
+      if (p.w) w[k].load(p.w, col);
+      if (p.b) b[k].load(p.b, col);
+    }
+  }
+  R raw[NV];
+  auto load = [&](int64_t row) {
+    const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int col = (t + k * lanes) * VEC;
+      raw[k] = row < p.rows && col < p.width ? load_once<R>(x + col) : raw_zero<R>();
+    }
+  };
+  int64_t row = (int64_t)blockIdx.x * groups + (LANES ? threadIdx.x / lanes : 0);
+  load(row);
+  int half = 0;
+  // Every group takes the same number of turns, so the block's barriers match.
+  for (int64_t base = (int64_t)blockIdx.x * groups; base < p.rows; base += stride, row += stride, half ^= 1) {
+    using V = typename Lanes<VEC>::V;
+    constexpr int NP = Lanes<VEC>::N;
+    V v[NV][NP], acc = vset(V{}, 0.f);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      unpack_lanes<T, VEC>(raw[k], v[k]);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) acc = vadd(acc, v[k][i]);
+    }
+    load(row + stride);
+    const float mean = row_sum<LANES>(hsum(acc), scratch[half]) * inv;
+    const V minus = vset(V{}, -mean);
+    acc = vset(V{}, 0.f);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const bool in = (t + k * lanes) * VEC < p.width;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        v[k][i] = vadd(v[k][i], minus);
+        if (in) acc = vfma(v[k][i], v[k][i], acc);
+      }
+    }
+    const float rstd = rsqrtf(row_sum<LANES>(hsum(acc), scratch[half] + 1) * inv + p.eps);
+    if (row >= p.rows) continue;
+    if (t == 0) {
+      if (p.mean) p.mean[row] = mean;
+      if (p.rstd) p.rstd[row] = rstd;
+    }
+    T* y = static_cast<T*>(p.y) + row * p.y_ld;
+    const V scale = vset(V{}, rstd);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int col = (t + k * lanes) * VEC;
+      if (col >= p.width) continue;
+      V f[NP];
+      if constexpr (!HELD) {
+        if (p.w) w[0].load(p.w, col);
+        if (p.b) b[0].load(p.b, col);
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i) v[k][i] = vmul(v[k][i], scale);
+      if (p.w) {
+        w[HELD ? k : 0].get(f);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) v[k][i] = vmul(v[k][i], f[i]);
+      }
+      if (p.b) {
+        b[HELD ? k : 0].get(f);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) v[k][i] = vadd(v[k][i], f[i]);
+      }
+      store_once(y + col, pack_lanes<T, VEC>(v[k]));
+    }
+  }
+}
+
+// Longer rows: a warp per row (LANES = 32), or a CTA of a few warps (0), that holds its row as it
+// lies in memory, up to NV vectors a lane, and unpacks it for each of the three passes.  With
+// a whole row per warp the sums cost ten shuffles for up to 160 values a lane and there
+// are no barriers (5120 columns: 23 instructions a value with a CTA per row, about 8 here).
+// ROWS rows at a time share the weights' loads (which cost more than a 16-bit row's own, from L1)
+// and the barriers.
+template <typename T, typename TW, int VEC, int NV, int ROWS, int LANES, int MAXT, int PER_SM>
+__global__ void __launch_bounds__(MAXT, PER_SM) forward_row_kernel(const Fwd p) {
+  using R = Raw<T, VEC>;
+  using V = typename Lanes<VEC>::V;
+  constexpr int NP = Lanes<VEC>::N;
+  __shared__ float scratch[2 * ROWS][32];
+  const int lanes = LANES ? LANES : blockDim.x;
+  const int t = LANES ? threadIdx.x % (LANES ? LANES : 1) : threadIdx.x;
+  const int groups = LANES ? blockDim.x / lanes : 1;
+  const float inv = 1.0f / (float)p.width;
+  const int64_t row = ((int64_t)blockIdx.x * groups + (LANES ? threadIdx.x / lanes : 0)) * ROWS;
+  if (LANES && row >= p.rows) return;                // a whole warp
+  const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
+  R raw[ROWS][NV];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int col = (t + k * lanes) * VEC;
+      raw[r][k] = col < p.width && (r == 0 || row + r < p.rows) ? load_once<R>(x + r * p.x_ld + col) : raw_zero<R>();
+    }
+  float mean[ROWS], rstd[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    V acc = vset(V{}, 0.f);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      V v[NP];
+      unpack_lanes<T, VEC>(raw[r][k], v);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) acc = vadd(acc, v[i]);
+    }
+    mean[r] = hsum(acc);
+  }
+  row_sums<LANES>(mean, scratch);
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    mean[r] *= inv;
+    const V minus = vset(V{}, -mean[r]);
+    V acc = vset(V{}, 0.f);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      V v[NP];
+      unpack_lanes<T, VEC>(raw[r][k], v);
+      if ((t + k * lanes) * VEC < p.width) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const V d = vadd(v[i], minus);
+          acc = vfma(d, d, acc);
+        }
+      }
+    }
+    rstd[r] = hsum(acc);
+  }
+  row_sums<LANES>(rstd, scratch + ROWS);
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    rstd[r] = rsqrtf(rstd[r] * inv + p.eps);
+    if (t == 0 && row + r < p.rows) {
+      if (p.mean) p.mean[row + r] = mean[r];
+      if (p.rstd) p.rstd[row + r] = rstd[r];
+    }
   }
   T* y = static_cast<T*>(p.y) + row * p.y_ld;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int col = (t + k * lanes) * VEC;
-    if (col >= p.width) continue;
-    float w[VEC], b[VEC];
-    load_weight<TW, VEC>(p.w, col, 1.f, w);
-    load_weight<TW, VEC>(p.b, col, 0.f, b);
+    if (col >= p.width) break;
+    Weights<TW, VEC> w, b;
+    if (p.w) w.load(p.w, col);
+    if (p.b) b.load(p.b, col);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[k][i] = fmaf(v[k][i] * rstd, w[i], b[i]);
-    store_once(y + col, pack<T, VEC>(v[k]));
+    for (int r = 0; r < ROWS; ++r) {
+      if (r > 0 && row + r >= p.rows) break;
+      const V minus = vset(V{}, -mean[r]), scale = vset(V{}, rstd[r]);
+      V v[NP], f[NP];
+      unpack_lanes<T, VEC>(raw[r][k], v);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) v[i] = vmul(vadd(v[i], minus), scale);
+      if (p.w) {
+        w.get(f);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) v[i] = vmul(v[i], f[i]);
+      }
+      if (p.b) {
+        b.get(f);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) v[i] = vadd(v[i], f[i]);
+      }
+      store_once(y + r * p.y_ld + col, pack_lanes<T, VEC>(v));
+    }
   }
 }
 
@@ -141,12 +310,12 @@ __global__ void __launch_bounds__(1024) forward_wide_kernel(const Fwd p) {
   float sum = 0.f, sq = 0.f;
   for (int c = threadIdx.x; c < p.width; c += blockDim.x) sum += to_f32(x[c]);
   const float inv = 1.0f / (float)p.width;
-  const float mean = row_sum<0>(sum, scratch[0]) * inv;
+  const float mean = row_sum<0>(sum, scratch) * inv;
   for (int c = threadIdx.x; c < p.width; c += blockDim.x) {
     const float d = to_f32(x[c]) - mean;
     sq = fmaf(d, d, sq);
   }
-  const float rstd = rsqrtf(row_sum<0>(sq, scratch[1]) * inv + p.eps);
+  const float rstd = rsqrtf(row_sum<0>(sq, scratch + 1) * inv + p.eps);
   if (threadIdx.x == 0) {
     if (p.mean) p.mean[row] = mean;
     if (p.rstd) p.rstd[row] = rstd;
@@ -159,7 +328,7 @@ __global__ void __launch_bounds__(1024) forward_wide_kernel(const Fwd p) {
   }
 }
 
-template <typename T, typename TW, int VEC, int NV, int LANES, int MAXT, int PER_SM>
+template <typename T, typename TW, int VEC, int NV, int LANES, int MAXT, int PER_SM, bool HELD>
 __global__ void __launch_bounds__(MAXT, PER_SM) backward_kernel(const Bwd p) {
   using R = Raw<T, VEC>;
   __shared__ float scratch[2][2][32];
@@ -168,11 +337,28 @@ __global__ void __launch_bounds__(MAXT, PER_SM) backward_kernel(const Bwd p) {
   const int groups = LANES ? blockDim.x / lanes : 1;       // rows a CTA walks side by side
   const int group = LANES ? threadIdx.x / lanes : 0;
   const float inv = 1.0f / (float)p.width;
-  float dw[NV][VEC], db[NV][VEC];
+  using V = typename Lanes<VEC>::V;
+  constexpr int NP = Lanes<VEC>::N;
+  V dw[NV][NP], db[NV][NP];
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) dw[k][i] = db[k][i] = 0.f;
+    for (int i = 0; i < NP; ++i) dw[k][i] = db[k][i] = vset(V{}, 0.f);
+  Weights<TW, VEC> held[HELD ? NV : 1];
+  if constexpr (HELD) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (p.w && (t + k * lanes) * VEC < p.width) held[k].load(p.w, (t + k * lanes) * VEC);
+  }
+  auto weights = [&](int k, int col, V (&w)[NP]) {
+    if (p.w) {
+      if constexpr (!HELD) held[0].load(p.w, col);
+      held[HELD ? k : 0].get(w);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) w[i] = vset(V{}, 1.f);
+    }
+  };
 
   R rx[NV], rd[NV];
   float mean = 0.f, rstd = 0.f;
@@ -204,63 +390,44 @@ __global__ void __launch_bounds__(MAXT, PER_SM) backward_kernel(const Bwd p) {
       cd[k] = rd[k];
     }
     load(row + stride);
-    float s1 = 0.f, s2 = 0.f;
+    const V minus = vset(V{}, -m), scale = vset(V{}, r);
+    V a1 = vset(V{}, 0.f), a2 = vset(V{}, 0.f);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int col = (t + k * lanes) * VEC;
       if (col >= p.width) continue;
-      float x[VEC], d[VEC], w[VEC];
-      unpack<T, VEC>(cx[k], x);
-      unpack<T, VEC>(cd[k], d);
-      load_weight<TW, VEC>(p.w, col, 1.f, w);
+      V x[NP], d[NP], w[NP];
+      unpack_lanes<T, VEC>(cx[k], x);
+      unpack_lanes<T, VEC>(cd[k], d);
+      weights(k, col, w);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float xh = (x[i] - m) * r, td = w[i] * d[i];
-        s1 += td;
-        s2 = fmaf(td, xh, s2);
-        dw[k][i] = fmaf(d[i], xh, dw[k][i]);
-        db[k][i] += d[i];
+      for (int i = 0; i < NP; ++i) {
+        const V xh = vmul(vadd(x[i], minus), scale), td = vmul(w[i], d[i]);
+        a1 = vadd(a1, td);
+        a2 = vfma(td, xh, a2);
+        dw[k][i] = vfma(d[i], xh, dw[k][i]);
+        db[k][i] = vadd(db[k][i], d[i]);
       }
     }
-    if constexpr (LANES > 0) {
-      s1 = row_sum<LANES>(s1, nullptr);
-      s2 = row_sum<LANES>(s2, nullptr);
-    } else {              // both sums behind one barrier
-#pragma unroll
-      for (int o = 16; o; o >>= 1) {
-        s1 += __shfl_xor_sync(0xffffffffu, s1, o);
-        s2 += __shfl_xor_sync(0xffffffffu, s2, o);
-      }
-      if ((threadIdx.x & 31) == 0) {
-        scratch[half][0][threadIdx.x >> 5] = s1;
-        scratch[half][1][threadIdx.x >> 5] = s2;
-      }
-      __syncthreads();
-      s1 = s2 = 0.f;
-      const int warps = blockDim.x >> 5;
-      for (int w = 0; w < warps; ++w) {
-        s1 += scratch[half][0][w];
-        s2 += scratch[half][1][w];
-      }
-    }
+    float s[2] = {hsum(a1), hsum(a2)};
+    row_sums<LANES>(s, scratch[half]);
     if (row >= p.rows) continue;
-    s1 *= inv;
-    s2 *= inv;
+    const V c1 = vset(V{}, -s[0] * inv * r), c2 = vset(V{}, -s[1] * inv * r);
     T* dx = static_cast<T*>(p.dx) + row * p.dx_ld;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int col = (t + k * lanes) * VEC;
       if (col >= p.width) continue;
-      float x[VEC], d[VEC], w[VEC];
-      unpack<T, VEC>(cx[k], x);
-      unpack<T, VEC>(cd[k], d);
-      load_weight<TW, VEC>(p.w, col, 1.f, w);
+      V x[NP], d[NP], w[NP];
+      unpack_lanes<T, VEC>(cx[k], x);
+      unpack_lanes<T, VEC>(cd[k], d);
+      weights(k, col, w);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float xh = (x[i] - m) * r;
-        x[i] = r * (fmaf(w[i], d[i], -s1) - xh * s2);
+      for (int i = 0; i < NP; ++i) {
+        const V xh = vmul(vadd(x[i], minus), scale);
+        x[i] = vfma(xh, c2, vfma(vmul(w[i], d[i]), scale, c1));
       }
-      store_once(dx + col, pack<T, VEC>(x));
+      store_once(dx + col, pack_lanes<T, VEC>(x));
     }
   }
 
@@ -270,10 +437,13 @@ __global__ void __launch_bounds__(MAXT, PER_SM) backward_kernel(const Bwd p) {
     for (int k = 0; k < NV; ++k) {
       const int col = (t + k * lanes) * VEC;
       if (col >= p.width) continue;
+      float ew[VEC], eb[VEC];
+      from_lanes(dw[k], ew);
+      from_lanes(db[k], eb);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        part[col + i] = dw[k][i];
-        part[p.width + col + i] = db[k][i];
+        part[col + i] = ew[i];
+        part[p.width + col + i] = eb[i];
       }
     }
   } else {                // join the lane groups: column by column, groups in order
@@ -285,8 +455,10 @@ __global__ void __launch_bounds__(MAXT, PER_SM) backward_kernel(const Bwd p) {
       for (int k = 0; k < NV; ++k) {
         const int col = (t + k * lanes) * VEC;
         if (col >= p.width) continue;
+        float e[VEC];
+        from_lanes(which ? db[k] : dw[k], e);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) lines[group * p.width + col + i] = which ? db[k][i] : dw[k][i];
+        for (int i = 0; i < VEC; ++i) lines[group * p.width + col + i] = e[i];
       }
       __syncthreads();
       for (int c = threadIdx.x; c < p.width; c += blockDim.x) {
@@ -296,6 +468,196 @@ __global__ void __launch_bounds__(MAXT, PER_SM) backward_kernel(const Bwd p) {
       }
     }
   }
+}
+
+// Long rows whose start and length are multiples of 16 bytes: bulk copies stream x and dy rows
+// into a ring of shared memory (no addresses, predicates or registers per thread), ROWS rows
+// a stage.  Both passes read the stage; one barrier per stage joins the rows' sums, and
+// behind it the stage before is free: thread 0 refills it there.
+template <int N>
+__device__ __forceinline__ void warp_scatter_sum(float (&v)[N], int lane) {   // N = 2 or 4: lane holds sum lane / (32 / N)
+#pragma unroll
+  for (int n = N, o = 16; n > 1; n >>= 1, o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int j = 0; j < n / 2; ++j) {
+      const float send = up ? v[j] : v[j + n / 2], keep = up ? v[j + n / 2] : v[j];
+      v[j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+  }
+#pragma unroll
+  for (int o = 16 / N; o; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+}
+
+constexpr int kMaxStages = 4;
+
+template <typename T, typename TW, int VEC, int NV, int ROWS, int MAXT, int PER_SM, bool HELD>
+__global__ void __launch_bounds__(MAXT, PER_SM) backward_ring_kernel(const Bwd p, const int stages) {
+  using namespace sm100;
+  using R = Raw<T, VEC>;
+  using V = typename Lanes<VEC>::V;
+  constexpr int NP = Lanes<VEC>::N, SUMS = 2 * ROWS, SHARE = 32 / SUMS;
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ uint64_t full[kMaxStages];
+  __shared__ float scratch[2][SUMS][33];
+  __shared__ int given_up;
+  const int lanes = blockDim.x, warps = lanes >> 5;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const uint32_t row_bytes = p.width * sizeof(T), stage_bytes = 2 * ROWS * row_bytes;
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  auto fill = [&](int stage, int64_t row) {                  // one thread
+    if (row >= p.rows) return;
+    const int n = row + ROWS <= p.rows ? ROWS : (int)(p.rows - row);
+    mbar_arrive_expect_tx(&full[stage], 2 * n * row_bytes);
+    uint8_t* to = ring + (size_t)stage * stage_bytes;
+    for (int r = 0; r < n; ++r) {
+      bulk_load(to + 2 * r * row_bytes, static_cast<const T*>(p.x) + (row + r) * p.x_ld, row_bytes, &full[stage]);
+      bulk_load(to + (2 * r + 1) * row_bytes, static_cast<const T*>(p.dy) + (row + r) * p.dy_ld, row_bytes, &full[stage]);
+    }
+  };
+  int64_t row = (int64_t)blockIdx.x * ROWS;
+  if (t == 0) {
+    for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+    given_up = 0;
+    fence_barrier_init();
+    for (int s = 0; s < stages; ++s) fill(s, row + s * step);
+  }
+  for (int i = t; i < 2 * SUMS * 33; i += lanes) (&scratch[0][0][0])[i] = 0.f;   // warps that are not there count zero
+  __syncthreads();
+
+  const float inv = 1.0f / (float)p.width;
+  V dw[NV][NP], db[NV][NP];
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < NP; ++i) dw[k][i] = db[k][i] = vset(V{}, 0.f);
+  Weights<TW, VEC> held[HELD ? NV : 1];
+  if constexpr (HELD) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (p.w && (t + k * lanes) * VEC < p.width) held[k].load(p.w, (t + k * lanes) * VEC);
+  }
+  auto weights = [&](int k, int col, V (&w)[NP]) {
+    if (p.w) {
+      if constexpr (!HELD) held[0].load(p.w, col);
+      held[HELD ? k : 0].get(w);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) w[i] = vset(V{}, 1.f);
+    }
+  };
+  float mean[ROWS], rstd[ROWS];
+  auto stats = [&](int64_t row) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      mean[r] = row + r < p.rows ? __ldg(p.mean + row + r) : 0.f;
+      rstd[r] = row + r < p.rows ? __ldg(p.rstd + row + r) : 0.f;
+    }
+  };
+  stats(row);
+  int stage = 0, half = 0;
+  uint32_t phase = 0;
+  for (; row < p.rows; row += step, half ^= 1) {
+    int ok = mbar_wait(&full[stage], phase, &given_up);
+    const uint8_t* from = ring + (size_t)stage * stage_bytes;
+    const int n = row + ROWS <= p.rows ? ROWS : (int)(p.rows - row);
+    float sums[SUMS], m[ROWS], q[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      m[r] = mean[r];
+      q[r] = rstd[r];
+      V a1 = vset(V{}, 0.f), a2 = vset(V{}, 0.f);
+      if (r < n) {
+        const V minus = vset(V{}, -m[r]), scale = vset(V{}, q[r]);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          const int col = (t + k * lanes) * VEC;
+          if (col >= p.width) break;
+          V x[NP], d[NP], w[NP];
+          unpack_lanes<T, VEC>(*reinterpret_cast<const R*>(from + 2 * r * row_bytes + col * sizeof(T)), x);
+          unpack_lanes<T, VEC>(*reinterpret_cast<const R*>(from + (2 * r + 1) * row_bytes + col * sizeof(T)), d);
+          weights(k, col, w);
+#pragma unroll
+          for (int i = 0; i < NP; ++i) {
+            const V xh = vmul(vadd(x[i], minus), scale), td = vmul(w[i], d[i]);
+            a1 = vadd(a1, td);
+            a2 = vfma(td, xh, a2);
+            dw[k][i] = vfma(d[i], xh, dw[k][i]);
+            db[k][i] = vadd(db[k][i], d[i]);
+          }
+        }
+      }
+      sums[2 * r] = hsum(a1);
+      sums[2 * r + 1] = hsum(a2);
+    }
+    stats(row + step);                                       // of the next stage, while this one is joined
+    warp_scatter_sum(sums, lane);
+    if (lane % SHARE == 0) scratch[half][lane / SHARE][warp] = sums[0];
+    ok = __syncthreads_and(ok);                              // every warp has data, or all stop together
+    if (!ok) {
+      if (t == 0) {                                          // copies already issued land before the CTA exits
+        const uint64_t t0 = globaltimer();
+        for (int i = 0; i < stages && row < p.rows; ++i, row += step) {
+          while (!mbar_try_wait(&full[stage], phase) && globaltimer() - t0 < kWaitLimitNs) {
+          }
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      break;
+    }
+    if (t == 0 && row != (int64_t)blockIdx.x * ROWS) fill(stage ? stage - 1 : stages - 1, row + (stages - 1) * step);
+    float s = 0.f;                                           // sum lane / SHARE over the warps
+#pragma unroll
+    for (int w = 0; w < 32; w += SHARE)
+      if (w < warps) s += scratch[half][lane / SHARE][w + lane % SHARE];
+#pragma unroll
+    for (int o = SHARE / 2; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const float s1 = __shfl_sync(0xffffffffu, s, 2 * r * SHARE), s2 = __shfl_sync(0xffffffffu, s, (2 * r + 1) * SHARE);
+      if (r >= n) continue;
+      const V minus = vset(V{}, -m[r]), scale = vset(V{}, q[r]);
+      const V c1 = vset(V{}, -s1 * inv * q[r]), c2 = vset(V{}, -s2 * inv * q[r]);
+      T* dx = static_cast<T*>(p.dx) + (row + r) * p.dx_ld;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int col = (t + k * lanes) * VEC;
+        if (col >= p.width) break;
+        V x[NP], d[NP], w[NP];
+        unpack_lanes<T, VEC>(*reinterpret_cast<const R*>(from + 2 * r * row_bytes + col * sizeof(T)), x);
+        unpack_lanes<T, VEC>(*reinterpret_cast<const R*>(from + (2 * r + 1) * row_bytes + col * sizeof(T)), d);
+        weights(k, col, w);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const V xh = vmul(vadd(x[i], minus), scale);
+          x[i] = vfma(xh, c2, vfma(vmul(w[i], d[i]), scale, c1));
+        }
+        store_once(dx + col, pack_lanes<T, VEC>(x));
+      }
+    }
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+  float* part = p.part + (int64_t)blockIdx.x * 2 * p.width;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int col = (t + k * lanes) * VEC;
+    if (col >= p.width) break;
+    float ew[VEC], eb[VEC];
+    from_lanes(dw[k], ew);
+    from_lanes(db[k], eb);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      part[col + i] = ew[i];
+      part[p.width + col + i] = eb[i];
+    }
+  }
+  if (given_up && t == 0 && p.status) atomicExch(p.status, VDN_ERR_TIMEOUT);
 }
 
 // Any width: dx by a CTA per row, and the column sums by a CTA per 256 columns and row chunk.
@@ -313,8 +675,8 @@ __global__ void __launch_bounds__(1024) backward_wide_kernel(const Bwd p) {
     s1 += td;
     s2 = fmaf(td, (to_f32(x[c]) - m) * r, s2);
   }
-  s1 = row_sum<0>(s1, scratch[0]) * inv;
-  s2 = row_sum<0>(s2, scratch[1]) * inv;
+  s1 = row_sum<0>(s1, scratch) * inv;
+  s2 = row_sum<0>(s2, scratch + 1) * inv;
   T* dx = static_cast<T*>(p.dx) + row * p.dx_ld;
   for (int c = threadIdx.x; c < p.width; c += blockDim.x) {
     const float xh = (to_f32(x[c]) - m) * r;
@@ -338,69 +700,144 @@ __global__ void __launch_bounds__(256) columns_wide_kernel(const Bwd p) {
   part[p.width + c] = db;
 }
 
-template <typename T, typename TW, int VEC, int NV, int LANES, int MAXT>
+constexpr int kSMs = 148;
+
+template <typename T, typename TW, int VEC, int NV, int LANES, int MAXT, int PER_SM, bool HELD>
 static int launch_forward(const Fwd& p, int block, cudaStream_t stream) {
   const int64_t per = LANES ? block / (LANES ? LANES : 1) : 1;
-  forward_kernel<T, TW, VEC, NV, LANES, MAXT><<<(unsigned)((p.rows + per - 1) / per), block, 0, stream>>>(p);
+  const int64_t ctas = (p.rows + per - 1) / per, most = kSMs * (LANES || block * 2 > MAXT ? PER_SM : 2 * PER_SM);
+  forward_kernel<T, TW, VEC, NV, LANES, MAXT, PER_SM, HELD><<<(unsigned)(ctas < most ? ctas : most), block, 0, stream>>>(p);
   VDN_LAUNCH_CHECK("layer norm");
   return VDN_OK;
+}
+
+template <typename T, typename TW, int VEC, int NV, int ROWS, int LANES, int MAXT, int PER_SM>
+static int launch_row(const Fwd& p, int block, cudaStream_t stream) {
+  const int64_t per = (LANES ? block / (LANES ? LANES : 1) : 1) * ROWS;
+  forward_row_kernel<T, TW, VEC, NV, ROWS, LANES, MAXT, PER_SM><<<(unsigned)((p.rows + per - 1) / per), block, 0, stream>>>(p);
+  VDN_LAUNCH_CHECK("layer norm (rows)");
+  return VDN_OK;
+}
+
+// Elements per access that the width, the strides and the addresses allow: 16 bytes, 4, or one.
+template <typename T>
+static int vector_of(int width, std::initializer_list<int64_t> strides, std::initializer_list<const void*> rows,
+                     std::initializer_list<const void*> params, size_t param_size) {
+  for (int v : {16 / (int)sizeof(T), 2}) {
+    bool ok = width % v == 0;
+    for (int64_t s : strides) ok = ok && s % v == 0;
+    for (const void* q : rows) ok = ok && aligned_to(q, v * sizeof(T));
+    for (const void* q : params) ok = ok && (!q || aligned_to(q, v * param_size > 16 ? 16 : v * param_size));
+    if (ok) return v;
+  }
+  return 1;
 }
 
 template <typename T, typename TW>
 static int forward(const Fwd& p, cudaStream_t stream) {
   constexpr int V = 16 / sizeof(T);
-  const size_t wv = sizeof(TW) * V > 16 ? 16 : sizeof(TW) * V;
-  const bool vec = p.width % V == 0 && p.x_ld % V == 0 && p.y_ld % V == 0 && aligned16(p.x) && aligned16(p.y) &&
-                   (!p.w || aligned_to(p.w, wv)) && (!p.b || aligned_to(p.b, wv));
-  if (vec) {
-    const int n = p.width / V;
-    if (n <= 8) return launch_forward<T, TW, V, 1, 8, 256>(p, 256, stream);
-    if (n <= 16) return launch_forward<T, TW, V, 1, 16, 256>(p, 256, stream);
-    if (n <= 32) return launch_forward<T, TW, V, 1, 32, 256>(p, 256, stream);
-    if (n <= 64) return launch_forward<T, TW, V, 2, 32, 256>(p, 256, stream);
-    if (n <= 128) return launch_forward<T, TW, V, 4, 32, 256>(p, 256, stream);
-    if (n <= 2 * 512) return launch_forward<T, TW, V, 2, 0, 512>(p, (n + 63) / 64 * 32, stream);
-    if (n <= 4 * 1024) return launch_forward<T, TW, V, 4, 0, 1024>(p, (n + 127) / 128 * 32, stream);
+  const int vec = vector_of<T>(p.width, {p.x_ld, p.y_ld}, {p.x, p.y}, {p.w, p.b}, sizeof(TW));
+  const int n = p.width / vec;
+  if (vec == V) {
+    if (n <= 8) return launch_forward<T, TW, V, 1, 8, 256, 5, true>(p, 256, stream);
+    if (n <= 16) return launch_forward<T, TW, V, 1, 16, 256, 5, true>(p, 256, stream);
+    if (n <= 32) return launch_forward<T, TW, V, 1, 32, 256, 5, true>(p, 256, stream);
+    // 16-bit rows under fp32 weights are bound by the weights' loads: two rows share them.
+    if (sizeof(T) == 2) {
+      if (n <= 2 * 32) return launch_row<T, TW, V, 2, 2, 32, 128, 8>(p, 128, stream);
+      if (n <= 4 * 32) return launch_row<T, TW, V, 4, 2, 32, 128, 6>(p, 128, stream);
+      if (n <= 5 * 256) return launch_row<T, TW, V, 5, 2, 0, 256, 2>(p, (n + 159) / 160 * 32, stream);
+      if (n <= 8 * 256) return launch_row<T, TW, V, 8, 1, 0, 256, 3>(p, (n + 255) / 256 * 32, stream);
+      if (n <= 8 * 1024) return launch_row<T, TW, V, 8, 1, 0, 1024, 1>(p, (n + 255) / 256 * 32, stream);
+    } else {
+      if (n <= 4 * 32) return launch_row<T, TW, V, 4, 1, 32, 256, 4>(p, 256, stream);
+      if (n <= 8 * 32) return launch_row<T, TW, V, 8, 1, 32, 256, 3>(p, 256, stream);
+      if (n <= 12 * 128) return launch_row<T, TW, V, 12, 1, 0, 512, 1>(p, (n + 383) / 384 * 32, stream);
+      if (n <= 4 * 1024) return launch_row<T, TW, V, 4, 1, 0, 1024, 1>(p, (n + 127) / 128 * 32, stream);
+      if (n <= 12 * 512) return launch_row<T, TW, V, 12, 1, 0, 512, 1>(p, (n + 383) / 384 * 32, stream);
+    }
+  } else if (vec == 2) {
+    if (n <= 8 * 32) return launch_row<T, TW, 2, 8, 1, 32, 256, 4>(p, 256, stream);
+    if (n <= 24 * 32) return launch_row<T, TW, 2, 24, 1, 32, 256, 3>(p, 256, stream);
+    if (n <= 16 * 1024) return launch_row<T, TW, 2, 16, 1, 0, 1024, 1>(p, (n + 511) / 512 * 32, stream);
   } else {
-    if (p.width <= 128) return launch_forward<T, TW, 1, 4, 32, 256>(p, 256, stream);
-    if (p.width <= 8 * 512) return launch_forward<T, TW, 1, 8, 0, 512>(p, (p.width + 255) / 256 * 32, stream);
-    if (p.width <= 16 * 1024) return launch_forward<T, TW, 1, 16, 0, 1024>(p, (p.width + 511) / 512 * 32, stream);
+    if (n <= 8 * 32) return launch_row<T, TW, 1, 8, 1, 32, 256, 4>(p, 256, stream);
+    if (n <= 24 * 32) return launch_row<T, TW, 1, 24, 1, 32, 256, 3>(p, 256, stream);
+    if (n <= 16 * 1024) return launch_row<T, TW, 1, 16, 1, 0, 1024, 1>(p, (n + 511) / 512 * 32, stream);
   }
   forward_wide_kernel<T, TW><<<(unsigned)p.rows, 1024, 0, stream>>>(p);
   VDN_LAUNCH_CHECK("layer norm (wide)");
   return VDN_OK;
 }
 
-// CTAs of the backward, one line of partial sums each: enough to fill 148 SMs a few times
-// over for short rows; the count depends on the shape alone, so results do not vary.
-constexpr int kLines = 296;
+// CTAs of the backward, one line of partial sums each.  A CTA per row has about width / 16
+// threads, so narrower rows take more CTAs to fill 148 SMs.  The count depends on the
+// shape alone, so results do not vary.
+static int64_t line_count(int64_t rows, int64_t width) {
+  const int64_t lines = 2 * kSMs * (width >= 5120 ? 1 : width <= 512 ? 10 : 5120 / width);
+  return rows < lines ? rows : lines;
+}
+constexpr int kGroupLines = 4 * kSMs;        // where a lane group takes a row: CTAs of several rows
 
-template <typename T, typename TW, int VEC, int NV, int LANES, int MAXT, int PER_SM>
+template <typename T, typename TW, int VEC, int NV, int LANES, int MAXT, int PER_SM, bool HELD>
 static int launch_backward(const Bwd& p, int block, int lines, cudaStream_t stream) {
   const size_t smem = LANES ? sizeof(float) * (block / (LANES ? LANES : 1)) * (size_t)p.width : 0;
-  backward_kernel<T, TW, VEC, NV, LANES, MAXT, PER_SM><<<lines, block, smem, stream>>>(p);
+  backward_kernel<T, TW, VEC, NV, LANES, MAXT, PER_SM, HELD><<<lines, block, smem, stream>>>(p);
   VDN_LAUNCH_CHECK("layer norm backward");
+  return VDN_OK;
+}
+
+// The ring kernel, where two stages fit beside the CTAs that share an SM (0: they do not).
+constexpr int kSmemPerSM = 227 * 1024;
+template <typename T, typename TW, int VEC, int NV, int ROWS, int MAXT, int PER_SM, bool HELD>
+static int launch_ring(const Bwd& p, int block, int lines, cudaStream_t stream, bool& done) {
+  const int share = PER_SM * (MAXT / block < 1 ? 1 : MAXT / block);   // CTAs an SM, by their threads
+  const int64_t stage = 2ll * ROWS * p.width * sizeof(T), room = kSmemPerSM / (share < 12 ? share : 12) - 2048;
+  const int stages = (int)(room / stage < kMaxStages ? room / stage : kMaxStages);
+  if (stages < 2) return VDN_OK;
+  auto* kernel = backward_ring_kernel<T, TW, VEC, NV, ROWS, MAXT, PER_SM, HELD>;
+  static bool set[64] = {};
+  int dev = 0;
+  VDN_CUDA_TRY(cudaGetDevice(&dev));
+  VDN_CHECK_ARG(dev >= 0 && dev < 64, "device index out of range");
+  if (!set[dev]) {
+    VDN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemPerSM - 4096));
+    set[dev] = true;
+  }
+  kernel<<<lines, block, stages * stage, stream>>>(p, stages);
+  VDN_LAUNCH_CHECK("layer norm backward (ring)");
+  done = true;
   return VDN_OK;
 }
 
 template <typename T, typename TW>
 static int backward(const Bwd& p, int lines, void* dw, void* db, cudaStream_t stream) {
   constexpr int V = 16 / sizeof(T), M = sizeof(T) / 2;   // M: fp32 holds half the values per vector
-  const size_t wv = sizeof(TW) * V > 16 ? 16 : sizeof(TW) * V;
-  const bool vec = p.width % V == 0 && p.x_ld % V == 0 && p.dy_ld % V == 0 && p.dx_ld % V == 0 && aligned16(p.x) &&
-                   aligned16(p.dy) && aligned16(p.dx) && (!p.w || aligned_to(p.w, wv));
-  const int n = p.width / V;
+  const int vec = vector_of<T>(p.width, {p.x_ld, p.dy_ld, p.dx_ld}, {p.x, p.dy, p.dx}, {p.w}, sizeof(TW));
+  const int n = p.width / vec, few = lines < kGroupLines ? lines : kGroupLines;
   int rc = -1;
-  if (vec) {
-    if (n <= 8) rc = launch_backward<T, TW, V, 1, 8, 256, 2>(p, 256, lines, stream);
-    else if (n <= 16) rc = launch_backward<T, TW, V, 1, 16, 256, 2>(p, 256, lines, stream);
-    else if (n <= 32) rc = launch_backward<T, TW, V, 1, 32, 256, 2>(p, 256, lines, stream);
-    else if (n <= 64) rc = launch_backward<T, TW, V, 2, 32, 128, 4>(p, 128, lines, stream);
-    else if (n <= 2 * M * 384) rc = launch_backward<T, TW, V, 2 * M, 0, 384, 2>(p, (n + 64 * M - 1) / (64 * M) * 32, lines, stream);
-    else if (n <= 4 * M * 512) rc = launch_backward<T, TW, V, 4 * M, 0, 512, 1>(p, (n + 128 * M - 1) / (128 * M) * 32, lines, stream);
+  if (vec == V) {
+    if (n <= 8) rc = launch_backward<T, TW, V, 1, 8, 128, 4, true>(p, 128, lines = few, stream);
+    else if (n <= 16) rc = launch_backward<T, TW, V, 1, 16, 128, 4, true>(p, 128, lines = few, stream);
+    else if (n <= 32) rc = launch_backward<T, TW, V, 1, 32, 128, 4, true>(p, 128, lines = few, stream);
+    else if (n <= 64) rc = launch_backward<T, TW, V, 2, 32, 128, 4, true>(p, 128, lines = few, stream);
+    else if (p.x_ld * sizeof(T) % 16 == 0 && p.dy_ld * sizeof(T) % 16 == 0) {   // (given by vec, said once more)
+      bool done = false;
+      int r = VDN_OK;
+      if (n <= 2 * M * 320) r = launch_ring<T, TW, V, 2 * M, 2 / M, 320, 2, true>(p, (n + 64 * M - 1) / (64 * M) * 32, lines, stream, done);
+      else if (n <= 4 * M * 512) r = launch_ring<T, TW, V, 4 * M, 1, 512, 1, false>(p, (n + 128 * M - 1) / (128 * M) * 32, lines, stream, done);
+      if (r != VDN_OK) return r;
+      if (done) rc = VDN_OK;
+    }
+    if (rc == VDN_OK) {
+    } else if (n <= 2 * M * 320) rc = launch_backward<T, TW, V, 2 * M, 0, 320, 2, sizeof(T) == 2>(p, (n + 64 * M - 1) / (64 * M) * 32, lines, stream);
+    else if (n <= 4 * M * 512) rc = launch_backward<T, TW, V, 4 * M, 0, 512, 1, false>(p, (n + 128 * M - 1) / (128 * M) * 32, lines, stream);
+  } else if (vec == 2) {
+    if (n <= 128) rc = launch_backward<T, TW, 2, 4, 32, 128, 4, true>(p, 128, lines = few, stream);
+    else if (n <= 8 * 512) rc = launch_backward<T, TW, 2, 8, 0, 512, 1, true>(p, (n + 255) / 256 * 32, lines, stream);
   } else {
-    if (p.width <= 128) rc = launch_backward<T, TW, 1, 4, 32, 128, 4>(p, 128, lines, stream);
-    else if (p.width <= 16 * 512) rc = launch_backward<T, TW, 1, 16, 0, 512, 1>(p, (p.width + 511) / 512 * 32, lines, stream);
+    if (n <= 256) rc = launch_backward<T, TW, 1, 8, 32, 128, 4, true>(p, 128, lines = few, stream);
+    else if (n <= 16 * 512) rc = launch_backward<T, TW, 1, 16, 0, 512, 1, true>(p, (n + 511) / 512 * 32, lines, stream);
   }
   if (rc > 0) return rc;
   if (rc < 0) {
@@ -447,15 +884,14 @@ extern "C" int vdn_layer_norm(const void* x, int dtype, int64_t rows, int64_t wi
 
 extern "C" size_t vdn_layer_norm_backward_workspace_size(int64_t rows, int64_t width) {
   if (rows < 1 || width < 1) return 0;
-  const int64_t lines = rows < vdn::lnorm::kLines ? rows : vdn::lnorm::kLines;
-  return sizeof(float) * 2 * (size_t)lines * (size_t)width;
+  return sizeof(float) * 2 * (size_t)vdn::lnorm::line_count(rows, width) * (size_t)width;
 }
 
 extern "C" int vdn_layer_norm_backward(const void* dy, int dtype, int64_t rows, int64_t width, int64_t dy_stride,
                                        const void* x, int64_t x_stride, const void* weight, int w_dtype,
                                        const float* mean, const float* rstd, void* dx, int64_t dx_stride,
                                        void* d_weight, void* d_bias, void* workspace, size_t workspace_bytes,
-                                       cudaStream_t stream) {
+                                       int* status, cudaStream_t stream) {
   using namespace vdn::lnorm;
   if (int rc = check(dtype, w_dtype, rows, width)) return rc;
   if (rows == 0) {
@@ -468,8 +904,8 @@ extern "C" int vdn_layer_norm_backward(const void* dy, int dtype, int64_t rows, 
   VDN_CHECK_ARG(rows == 1 || (dy_stride >= 0 && x_stride >= 0 && dx_stride >= width), "bad row stride");
   VDN_CHECK_ARG(workspace_bytes >= vdn_layer_norm_backward_workspace_size(rows, width),
                 "workspace smaller than vdn_layer_norm_backward_workspace_size");
-  const int lines = (int)(rows < kLines ? rows : kLines);
+  const int lines = (int)line_count(rows, width);
   const Bwd p = {dy, x, weight, mean, rstd, dx, static_cast<float*>(workspace), rows, dy_stride, x_stride, dx_stride,
-                 (int)width};
+                 (int)width, status};
   VDN_LN_DISPATCH(backward, p, lines, d_weight, d_bias, stream)
 }

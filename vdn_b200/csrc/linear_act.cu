@@ -82,13 +82,6 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t base, int ks) {
   return MN ? desc_mn_sw128(base + ks * 2048, 8192) : desc_k_sw128(base + ks * 32);
 }
 
-template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) { return pack_bf16x2(a, b); }
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 struct Params {
   const void* bias;      // [cols] or null
   const void* resid;     // [rows, cols], row stride ldr, or null

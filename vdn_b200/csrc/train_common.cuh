@@ -26,20 +26,105 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
+// A 32-bit word of two 16-bit values (the lower in the low half), and back with one conversion.
+template <typename T> __device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi);
+template <> __device__ __forceinline__ void unpack2<__nv_bfloat16>(uint32_t w, float& lo, float& hi) {
+  lo = __uint_as_float(w << 16);
+  hi = __uint_as_float(w & 0xFFFF0000u);
+}
+template <> __device__ __forceinline__ void unpack2<__half>(uint32_t w, float& lo, float& hi) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  lo = f.x;
+  hi = f.y;
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ void words(uint32_t r, uint32_t (&w)[1]) { w[0] = r; }
+__device__ __forceinline__ void words(const uint2& r, uint32_t (&w)[2]) { w[0] = r.x; w[1] = r.y; }
+__device__ __forceinline__ void words(const uint4& r, uint32_t (&w)[4]) { w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w; }
+__device__ __forceinline__ uint32_t join(const uint32_t (&w)[1]) { return w[0]; }
+__device__ __forceinline__ uint2 join(const uint32_t (&w)[2]) { return make_uint2(w[0], w[1]); }
+__device__ __forceinline__ uint4 join(const uint32_t (&w)[4]) { return make_uint4(w[0], w[1], w[2], w[3]); }
+
 template <typename T, int VEC>
 __device__ __forceinline__ void unpack(const Raw<T, VEC>& raw, float (&v)[VEC]) {
-  T e[VEC];
-  *reinterpret_cast<Raw<T, VEC>*>(e) = raw;
+  if constexpr (VEC == 1 && sizeof(T) == 2) {
+    T e;
+    *reinterpret_cast<uint16_t*>(&e) = raw;
+    v[0] = to_f32(e);
+  } else {
+    uint32_t w[VEC * sizeof(T) / 4];
+    words(raw, w);
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) v[i] = to_f32(e[i]);
+      for (int i = 0; i < VEC; ++i) v[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) unpack2<T>(w[i], v[2 * i], v[2 * i + 1]);
+    }
+  }
 }
 
 template <typename T, int VEC>
 __device__ __forceinline__ Raw<T, VEC> pack(const float (&v)[VEC]) {
-  alignas(16) T e[VEC];
+  if constexpr (VEC == 1 && sizeof(T) == 2) {
+    const T e = from_f32<T>(v[0]);
+    return *reinterpret_cast<const uint16_t*>(&e);
+  } else {
+    uint32_t w[VEC * sizeof(T) / 4];
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) e[i] = from_f32<T>(v[i]);
-  return *reinterpret_cast<Raw<T, VEC>*>(e);
+      for (int i = 0; i < VEC; ++i) w[i] = __float_as_uint(v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+    }
+    return join(w);
+  }
+}
+
+// Arithmetic on one value (float) or two (f2, packed fp32 pairs: one instruction for both).
+__device__ __forceinline__ float vset(float, float c) { return c; }
+__device__ __forceinline__ f2 vset(f2, float c) { return f2_pack(c, c); }
+__device__ __forceinline__ float vadd(float a, float b) { return a + b; }
+__device__ __forceinline__ f2 vadd(f2 a, f2 b) { return f2_add(a, b); }
+__device__ __forceinline__ float vmul(float a, float b) { return a * b; }
+__device__ __forceinline__ f2 vmul(f2 a, f2 b) { return f2_mul(a, b); }
+__device__ __forceinline__ float vfma(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ f2 vfma(f2 a, f2 b, f2 c) { return f2_fma(a, b, c); }
+template <int VEC> struct Lanes { using V = f2; static constexpr int N = VEC / 2; };
+template <> struct Lanes<1> { using V = float; static constexpr int N = 1; };
+
+__device__ __forceinline__ void spread(float a, float& v) { v = a; }
+__device__ __forceinline__ void spread(float a, f2& v) { v = f2_pack(a, a); }
+__device__ __forceinline__ void spread(f2 a, f2& v) { v = a; }
+
+__device__ __forceinline__ void to_lanes(const float (&e)[1], float (&v)[1]) { v[0] = e[0]; }
+template <int VEC> __device__ __forceinline__ void to_lanes(const float (&e)[VEC], f2 (&v)[VEC / 2]) {
+#pragma unroll
+  for (int i = 0; i < VEC / 2; ++i) v[i] = f2_pack(e[2 * i], e[2 * i + 1]);
+}
+__device__ __forceinline__ void from_lanes(const float (&v)[1], float (&e)[1]) { e[0] = v[0]; }
+template <int VEC> __device__ __forceinline__ void from_lanes(const f2 (&v)[VEC / 2], float (&e)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC / 2; ++i) f2_unpack(v[i], e[2 * i], e[2 * i + 1]);
+}
+template <typename T, int VEC, typename V, int N>
+__device__ __forceinline__ void unpack_lanes(const Raw<T, VEC>& raw, V (&v)[N]) {
+  float e[VEC];
+  unpack<T, VEC>(raw, e);
+  to_lanes(e, v);
+}
+template <typename T, int VEC, typename V, int N>
+__device__ __forceinline__ Raw<T, VEC> pack_lanes(const V (&v)[N]) {
+  float e[VEC];
+  from_lanes(v, e);
+  return pack<T, VEC>(e);
 }
 
 template <typename R> __device__ __forceinline__ R raw_zero() { return R{}; }
@@ -50,22 +135,24 @@ template <typename R> __device__ __forceinline__ void store_once(void* p, const 
 
 inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
-// Sums `lines` lines of `cols` fp32 partial sums in a fixed order: 32 columns by 8 line
+// Sums `lines` lines of `cols` fp32 partial sums in a fixed order: 32 columns by 32 line
 // groups a block.  Columns below `split` go to `a`, the others to `b` (either may be null).
 template <typename T>
-__global__ void __launch_bounds__(256) lines_kernel(const float* part, int lines, int64_t cols, T* a, int64_t split,
-                                                    T* b) {
-  __shared__ float sums[8][33];
+__global__ void __launch_bounds__(1024) lines_kernel(const float* part, int lines, int64_t cols, T* a, int64_t split,
+                                                     T* b) {
+  __shared__ float sums[32][33];
   const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
   float s = 0.f;
-  if (c < cols)
-    for (int l = g; l < lines; l += 8) s += part[l * cols + c];
+  if (c < cols) {
+#pragma unroll 4
+    for (int l = g; l < lines; l += 32) s += part[l * cols + c];
+  }
   sums[g][lane] = s;
   __syncthreads();
   if (g == 0 && c < cols) {
 #pragma unroll
-    for (int k = 1; k < 8; ++k) s += sums[k][lane];
+    for (int k = 1; k < 32; ++k) s += sums[k][lane];
     if (c < split) {
       if (a) a[c] = from_f32<T>(s);
     } else if (b) {
@@ -75,7 +162,7 @@ __global__ void __launch_bounds__(256) lines_kernel(const float* part, int lines
 }
 template <typename T>
 inline int add_lines(const float* part, int lines, int64_t cols, T* a, int64_t split, T* b, cudaStream_t stream) {
-  lines_kernel<T><<<(unsigned)((cols + 31) / 32), 256, 0, stream>>>(part, lines, cols, a, split, b);
+  lines_kernel<T><<<(unsigned)((cols + 31) / 32), 1024, 0, stream>>>(part, lines, cols, a, split, b);
   VDN_LAUNCH_CHECK("line sums");
   return VDN_OK;
 }

@@ -15,6 +15,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
+from .mxfp8_linear import _status
 
 __all__ = ["layer_norm", "layer_norm_backward"]
 
@@ -120,7 +121,8 @@ def _backward(grad_y, x, weight, mean, rstd, want_w, want_b, bias_dtype=None):
     mean, rstd = mean.contiguous(), rstd.contiguous()
     _lib.call_on(x.device, "vdn_layer_norm_backward", dy.data_ptr(), _lib.dtype_code(x.dtype), rows, width, dy_ld,
                  flat.data_ptr(), x_ld, _lib.address(w), _lib.dtype_code(kind), mean.data_ptr(), rstd.data_ptr(),
-                 dx.data_ptr(), width, _lib.address(dw), _lib.address(db), ws.data_ptr(), need)
+                 dx.data_ptr(), width, _lib.address(dw), _lib.address(db), ws.data_ptr(), need,
+                 _status(x.device).data_ptr())
     return dx, dw, db
 
 
