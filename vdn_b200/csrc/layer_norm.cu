@@ -619,8 +619,9 @@ __global__ void __launch_bounds__(MAXT, PER_SM) backward_ring_kernel(const Bwd p
     for (int r = 0; r < ROWS; ++r) {
       const float s1 = __shfl_sync(0xffffffffu, s, 2 * r * SHARE), s2 = __shfl_sync(0xffffffffu, s, (2 * r + 1) * SHARE);
       if (r >= n) continue;
-      const V minus = vset(V{}, -m[r]), scale = vset(V{}, q[r]);
-      const V c1 = vset(V{}, -s1 * inv * q[r]), c2 = vset(V{}, -s2 * inv * q[r]);
+      // dx = q t - q s1 - q xh s2 with xh = (x - m) q: one scale and one offset per row
+      const float slope = -s2 * inv * q[r] * q[r];
+      const V scale = vset(V{}, q[r]), c2 = vset(V{}, slope), c1 = vset(V{}, fmaf(-m[r], slope, -s1 * inv * q[r]));
       T* dx = static_cast<T*>(p.dx) + (row + r) * p.dx_ld;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
@@ -632,8 +633,7 @@ __global__ void __launch_bounds__(MAXT, PER_SM) backward_ring_kernel(const Bwd p
         weights(k, col, w);
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-          const V xh = vmul(vadd(x[i], minus), scale);
-          x[i] = vfma(xh, c2, vfma(vmul(w[i], d[i]), scale, c1));
+          x[i] = vfma(x[i], c2, vfma(vmul(w[i], d[i]), scale, c1));
         }
         store_once(dx + col, pack_lanes<T, VEC>(x));
       }
