@@ -9,6 +9,9 @@
 // per channel and runs join in any grouping.  HBM is the bound: the forward moves three
 // elements per token and channel, the backward five, for a dozen instructions each.  So
 // the inputs are read ONCE and kept in registers while the runs are joined:
+//   * rows travel as tiles (L tokens of a warp's channels) by tensor-map copies, two rounds ahead,
+//     and results leave the same way from the tile they replace: no addresses or predicates
+//     per element (with plain loads the scan was bound by issue, half of it such overhead);
 //   * a warp owns L tokens of 32 * VEC channels (lane = VEC neighbouring channels) and folds
 //     them into (A, H), keeping for each token its state from zero and its reach, the
 //     product of the decays so far; after the join its true states are state + reach * carry;
@@ -32,6 +35,7 @@
 
 #include "train_common.cuh"
 #include "sm100.cuh"
+#include "tma_host.cuh"
 
 namespace vdn {
 namespace gscan {
@@ -116,19 +120,37 @@ __device__ __forceinline__ void send(uint32_t addr, const Fold<f2>& f, uint32_t 
                "l"(f.a), "l"(f.h), "r"(bar) : "memory");
 }
 
+// Where a warp's rows come from: ROWS_LOAD plain loads into registers (any stride and alignment);
+// ROWS_UP / ROWS_DOWN tensor-map copies into a ring of tiles in shared memory, token rows
+// ascending or descending along the walk.
+enum { ROWS_LOAD = 0, ROWS_UP = 1, ROWS_DOWN = 2 };
+constexpr int kStages = 2;
+
+struct Maps {
+  CUtensorMap x, g, y, out, dg;
+};
+
 template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED>
-__global__ void __launch_bounds__(MAX_WARPS * 32, 5) scan_kernel(const Params p, const int cluster) {
+constexpr int tile_bytes() {   // of one warp and stage: x (dy), the saved y, the decays
+  return 32 * VEC * L * ((BWD ? 2 : 1) * (int)sizeof(T) + (SHARED ? 0 : (int)sizeof(TG)));
+}
+
+template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED, int FROM>
+__global__ void __launch_bounds__(MAX_WARPS * 32, FROM == ROWS_LOAD ? 3 : 4)
+    scan_kernel(const Params p, const int cluster, const __grid_constant__ Maps maps) {
   constexpr int GV = SHARED ? 1 : VEC;               // decays per lane and token
   constexpr int TILE = 32 * VEC;
+  constexpr bool RING = FROM != ROWS_LOAD;
   using RX = Raw<T, VEC>;
   using RG = Raw<TG, GV>;
   using V = typename Lanes<VEC>::V;                  // values
   using G = typename Lanes<GV>::V;                   // decays
   constexpr int NV = Lanes<VEC>::N, NG = Lanes<GV>::N;
+  extern __shared__ __align__(128) uint8_t tiles[];  // RING: [warps][kStages][tile_bytes]
   __shared__ Fold<V> folds[2][MAX_WARPS][NV][32];
   __shared__ G sums[2][MAX_WARPS][NG][32];
   __shared__ Fold<V> runs[2][MAX_CLUSTER][NV][32];   // one line from every CTA of the cluster
-  __shared__ uint64_t arrived[2];
+  __shared__ uint64_t arrived[2], full[MAX_WARPS][kStages];
   __shared__ int given_up;
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -138,7 +160,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 5) scan_kernel(const Params p,
   const int tile = (int)(id - seq * p.tiles);
   const int64_t c = (int64_t)tile * TILE + lane * VEC;
   const bool live = c < p.channels;
-  const bool full = (int64_t)(tile + 1) * TILE <= p.channels;
+  const bool whole = (int64_t)(tile + 1) * TILE <= p.channels;
   const int64_t gc = SHARED ? tile : c;              // shared: one head is one tile
 
   int begin = 0, len = p.rows;
@@ -157,16 +179,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 5) scan_kernel(const Params p,
     return;                                          // the whole cluster is here
   }
 
-  if (threadIdx.x == 0) {
-    mbar_init(&arrived[0], 1);
-    mbar_init(&arrived[1], 1);
-    given_up = 0;
-    fence_barrier_init();
-  }
-  cluster_sync();                                    // the barriers stand before anyone sends
-
   // Walk order: the forward follows the recurrence, the backward its reverse.
-  const bool down = p.reverse != BWD;                // token rows descend along the walk
+  const bool down = RING ? FROM == ROWS_DOWN : p.reverse != BWD;   // token rows descend along the walk
   const int64_t row0 = down ? (int64_t)begin + len - 1 : begin;
   const int sgn = down ? -1 : 1;
   const int64_t b = p.cu ? 0 : seq;
@@ -187,42 +201,91 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 5) scan_kernel(const Params p,
     to_lanes(e, carry);
   }
 
-  RX rx[L], ry[BWD ? L : 1];
-  RG rg[L];
-  auto load = [&](int64_t i0) {
-    const T* qx = px + i0 * sx;
-    const TG* qg = pg + i0 * sg;
-    if (full && i0 + L + (BWD ? 1 : 0) <= len) {      // the common case, without predicates
-      const T* qy = BWD ? py + (i0 + 1) * sy : nullptr;
-#pragma unroll
-      for (int l = 0; l < L; ++l) {
-        rx[l] = load_once<RX>(qx + l * sx);
-        rg[l] = load_once<RG>(qg + l * sg);
-        if constexpr (BWD) ry[l] = load_once<RX>(qy + l * sy);
-      }
-      return;
-    }
-    const int n = live ? (int)min((int64_t)len - i0, (int64_t)L) : 0;
-    const int ng = SHARED ? (int)min((int64_t)len - i0, (int64_t)L) : n;
-#pragma unroll
-    for (int l = 0; l < L; ++l) {
-      rx[l] = l < n ? load_once<RX>(qx + l * sx) : raw_zero<RX>();
-      rg[l] = l < ng ? load_once<RG>(qg + l * sg) : raw_zero<RG>();
-    }
-    if constexpr (BWD) {
-      const T* qy = py + (i0 + 1) * sy;
-      const int ny = i0 + n == len ? n - 1 : n;      // the oldest token's h_{t-1} is the first state
-#pragma unroll
-      for (int l = 0; l < L; ++l) ry[l] = l < ny ? load_once<RX>(qy + l * sy) : raw_zero<RX>();
-    }
-  };
-
   const int round_tokens = cluster * warps * L;
   int64_t i0 = (rank * warps + warp) * L;
-  int buf = 0;
-  uint32_t phase = 0;
+
+  // Tiles: x, then the saved y, then the decays; a lane's VEC values of token row r at r * pitch.
+  constexpr int PX = TILE * sizeof(T), PG = TILE * sizeof(TG), BYTES = tile_bytes<T, TG, VEC, L, BWD, SHARED>();
+  uint8_t* ring = tiles + warp * kStages * BYTES;
+  auto copy = [&](int stage, int64_t i) {            // one lane: the rows of walk tokens i .. i + L - 1
+    if (i >= len) return;
+    const int r = (int)(down ? row0 - i - (L - 1) : row0 + i), x0 = tile * TILE;
+    uint8_t* to = ring + stage * BYTES;
+    uint64_t* bar = &full[warp][stage];
+    mbar_arrive_expect_tx(bar, BYTES);
+    tma_load_3d(to, &maps.x, bar, x0, r, (int)b);
+    if (BWD) tma_load_3d(to + L * PX, &maps.y, bar, x0, r + sgn, (int)b);   // the tokens before them
+    if (!SHARED) tma_load_3d(to + (BWD ? 2 : 1) * L * PX, &maps.g, bar, x0, r, (int)b);
+  };
+
+  if (threadIdx.x == 0) {
+    mbar_init(&arrived[0], 1);
+    mbar_init(&arrived[1], 1);
+    if (RING)
+      for (int w = 0; w < warps; ++w)
+        for (int s = 0; s < kStages; ++s) mbar_init(&full[w][s], 1);
+    given_up = 0;
+    fence_barrier_init();
+  }
+  cluster_sync();                                    // the barriers stand before anyone sends
+  if (RING && lane == 0)
+    for (int s = 0; s < kStages - 1; ++s) copy(s, i0 + (int64_t)s * round_tokens);
+
+  RX rx[RING ? 1 : L], ry[!RING && BWD ? L : 1];
+  RG rg[RING || SHARED ? 1 : L];
+  auto load = [&](int64_t i) {                       // ROWS_LOAD: a round's rows into registers
+    const T* qx = px + i * sx;
+    const TG* qg = pg + i * sg;
+    const int n = live ? (int)min((int64_t)len - i, (int64_t)L) : 0;
+#pragma unroll
+    for (int l = 0; l < L; ++l) {
+      rx[RING ? 0 : l] = l < n ? load_once<RX>(qx + l * sx) : raw_zero<RX>();
+      if (!SHARED) rg[RING || SHARED ? 0 : l] = l < n ? load_once<RG>(qg + l * sg) : raw_zero<RG>();
+    }
+    if constexpr (BWD) {
+      const T* qy = py + (i + 1) * sy;
+      const int ny = i + n == len ? n - 1 : n;       // the oldest token's h_{t-1} is the first state
+#pragma unroll
+      for (int l = 0; l < L; ++l) ry[RING ? 0 : l] = l < ny ? load_once<RX>(qy + l * sy) : raw_zero<RX>();
+    }
+  };
+  // Shared decays: lane l has token l's, one round ahead.
+  auto load_shared = [&](int64_t i) {
+    const bool in = lane < L && i + lane < len;
+    float e[1] = {0.f};
+    if (in) unpack<TG, 1>(*reinterpret_cast<const Raw<TG, 1>*>(pg + (i + lane) * sg), e);
+    return e[0];
+  };
+  float g_next = SHARED ? load_shared(i0) : 0.f;
+
+  int buf = 0, stage = 0;
+  uint32_t phase = 0, full_phase = 0;
   for (int64_t done = 0; done < len; done += round_tokens, i0 += round_tokens, buf ^= 1) {
-    load(i0);
+    const int n = (int)min((int64_t)len - i0, (int64_t)L);   // this warp's tokens; none or fewer at the end
+    const bool last_run = (int64_t)len - i0 <= L;    // the oldest token is among them (or none is)
+    int ok = 1;
+    uint8_t* at = ring + stage * BYTES + lane * (VEC * (int)sizeof(T));
+    uint8_t* at_g = ring + stage * BYTES + (BWD ? 2 : 1) * L * PX + lane * (GV * (int)sizeof(TG));
+    auto row = [](int l) { return FROM == ROWS_DOWN ? L - 1 - l : l; };
+    auto x_at = [&](int l) { return reinterpret_cast<RX*>(at + row(l) * PX); };
+    auto y_at = [&](int l) { return reinterpret_cast<RX*>(at + (L + row(l)) * PX); };
+    auto g_at = [&](int l) { return reinterpret_cast<RG*>(at_g + row(l) * PG); };
+    if constexpr (RING) {
+      if (n > 0) {
+        ok = mbar_wait(&full[warp][stage], full_phase, &given_up);
+        if (n < L) {                                 // rows of other sequences, or of none
+#pragma unroll
+          for (int l = 0; l < L; ++l)
+            if (l >= n) {
+              *x_at(l) = raw_zero<RX>();
+              if (!SHARED) *g_at(l) = raw_zero<RG>();
+            }
+        }
+      }
+    } else {
+      load(i0);
+    }
+
     // First walk, from zero: part[l] the state after token l, reach[l] the product of the
     // decays up to it, so that the true state is part + reach * (the carry).
     V part[L][NV], fold[NV];
@@ -234,32 +297,54 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 5) scan_kernel(const Params p,
       sum[v] = vset(G{}, 0.f);
       far[v] = vset(G{}, 1.f);
     }
+    float hi_lane = 1.f, lo_lane = 0.f;
+    if constexpr (SHARED) {
+      decay_pair(g_next, hi_lane, lo_lane);
+      float s = g_next;
 #pragma unroll
-    for (int l = 0; l < L; ++l) {
-      V x[NV];
-      G g[NG], hi[NG], lo[NG];
-      unpack_lanes<T, VEC>(rx[l], x);
-      unpack_lanes<TG, GV>(rg[l], g);
+      for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      sum[0] = vset(G{}, s);
+      g_next = load_shared(i0 + round_tokens);
+    }
+    if (!RING || n > 0) {
 #pragma unroll
-      for (int v = 0; v < NG; ++v) {
-        decay_pair(g[v], hi[v], lo[v]);
-        sum[v] = vadd(sum[v], g[v]);
-        far[v] = vmul(far[v], hi[v]);
-        reach[l][v] = far[v];
-      }
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        V h, e;
-        spread(hi[SHARED ? 0 : v], h);
-        spread(lo[SHARED ? 0 : v], e);
-        if (BWD) {
-          const V u = vadd(x[v], fold[v]);
-          fold[v] = vfma(h, u, vmul(e, u));
+      for (int l = 0; l < L; ++l) {
+        V x[NV];
+        G g[NG], hi[NG], lo[NG];
+        unpack_lanes<T, VEC>(RING ? *x_at(l) : rx[RING ? 0 : l], x);
+        if constexpr (SHARED) {
+          hi[0] = vset(G{}, __shfl_sync(0xffffffffu, hi_lane, l));
+          lo[0] = vset(G{}, __shfl_sync(0xffffffffu, lo_lane, l));
         } else {
-          fold[v] = vfma(h, fold[v], vfma(e, fold[v], x[v]));
+          unpack_lanes<TG, GV>(RING ? *g_at(l) : rg[RING || SHARED ? 0 : l], g);
         }
-        part[l][v] = fold[v];
+#pragma unroll
+        for (int v = 0; v < NG; ++v) {
+          if constexpr (!SHARED) {
+            decay_pair(g[v], hi[v], lo[v]);
+            sum[v] = vadd(sum[v], g[v]);
+          }
+          far[v] = vmul(far[v], hi[v]);
+          reach[l][v] = far[v];
+        }
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          V h, e;
+          spread(hi[SHARED ? 0 : v], h);
+          spread(lo[SHARED ? 0 : v], e);
+          if (BWD) {
+            const V u = vadd(x[v], fold[v]);
+            fold[v] = vfma(h, u, vmul(e, u));
+          } else {
+            fold[v] = vfma(h, fold[v], vfma(e, fold[v], x[v]));
+          }
+          part[l][v] = fold[v];
+        }
       }
+    }
+    if (RING && lane == 0) {                         // refill the stage before, once its results have left it
+      bulk_wait_group_read<0>();
+      copy(stage ? stage - 1 : kStages - 1, i0 + (int64_t)(kStages - 1) * round_tokens);
     }
 
     // Join the warps of the CTA: `before` is the fold of the warps in front of this one.
@@ -280,7 +365,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 5) scan_kernel(const Params p,
         before[v].h = vset(V{}, 0.f);
       }
     }
-    __syncthreads();
+    if (!__syncthreads_and(ok && !given_up)) break;  // a wait that gave up ends the whole CTA
 #pragma unroll
     for (int w = 0; w < MAX_WARPS - 1; ++w) {
       if (w < warp) {
@@ -314,7 +399,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 5) scan_kernel(const Params p,
     }
     // A line's buffer is written again two rounds later, by CTAs that have this one's next
     // line, which it sends after all its warps have read this round's.
-    if (!mbar_wait(&arrived[buf], phase, &given_up)) break;
+    mbar_wait(&arrived[buf], phase, &given_up);      // a failure ends the loop at the next round's barrier
     phase ^= buf;
     V in[NV];                                        // the true carry in front of this warp
 #pragma unroll
@@ -333,42 +418,38 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 5) scan_kernel(const Params p,
 #pragma unroll
     for (int v = 0; v < NV; ++v) in[v] = vfma(before[v].a, in[v], before[v].h);
 
-    // Second walk, with the true carry.
-    const int left = (int)min((int64_t)len - i0, (int64_t)L + 1);   // L + 1: more tokens follow
+    // Second walk, with the true carry.  A whole run of a ring takes the place of its inputs
+    // and leaves as it came; others are stored row by row.
     T* qo = po + i0 * so;
-    if constexpr (!BWD) {
-      auto walk = [&](auto all) {
+    TG* qdg = BWD ? pdg + i0 * sdg : nullptr;
+    float dgs[BWD && SHARED ? L : 1];
+    auto walk = [&](auto all, auto tile_out) {
+      V c0[NV];
 #pragma unroll
-        for (int l = 0; l < L; ++l) {
-          V y[NV];
+      for (int v = 0; v < NV; ++v) c0[v] = in[v];
+#pragma unroll
+      for (int l = 0; l < L; ++l) {
+        V y[NV];
+        const bool store = all.value || (live && l < n);
+        if constexpr (!BWD) {
 #pragma unroll
           for (int v = 0; v < NV; ++v) {
             V r;
             spread(reach[l][SHARED ? 0 : v], r);
             y[v] = vfma(r, in[v], part[l][v]);
           }
-          if (all.value || (live && l < left)) store_once(qo + l * so, pack_lanes<T, VEC>(y));
-        }
-      };
-      if (full && left >= L) walk(std::true_type{}); else walk(std::false_type{});
-    } else {
-      TG* qdg = pdg + i0 * sdg;
-      float dgs[L];
-      auto walk = [&](auto all) {
-        V c0[NV];
-#pragma unroll
-        for (int v = 0; v < NV; ++v) c0[v] = in[v];
-#pragma unroll
-        for (int l = 0; l < L; ++l) {
-          V u[NV], d[NV], y[NV];
-          unpack_lanes<T, VEC>(ry[l], y);
-          if (!all.value && l + 1 == left) {         // the oldest token
+          if constexpr (tile_out.value) *x_at(l) = pack_lanes<T, VEC>(y);
+          else if (store) store_once(qo + l * so, pack_lanes<T, VEC>(y));
+        } else {
+          V u[NV], d[NV];
+          unpack_lanes<T, VEC>(RING ? *y_at(l) : ry[RING ? 0 : l], y);
+          if (!all.value && last_run && l + 1 == n) {        // the oldest token
             float e[VEC];
 #pragma unroll
             for (int v = 0; v < VEC; ++v) e[v] = p.first && live ? p.first[seq * p.channels + c + v] : 0.f;
             to_lanes(e, y);
           }
-          unpack_lanes<T, VEC>(rx[l], u);
+          unpack_lanes<T, VEC>(RING ? *x_at(l) : rx[RING ? 0 : l], u);
 #pragma unroll
           for (int v = 0; v < NV; ++v) {
             V r;
@@ -377,38 +458,79 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 5) scan_kernel(const Params p,
             c0[v] = vfma(r, in[v], part[l][v]);
             d[v] = vmul(c0[v], y[v]);
           }
-          if (all.value || (live && l < left)) store_once(qo + l * so, pack_lanes<T, VEC>(u));
+          if constexpr (tile_out.value) *x_at(l) = pack_lanes<T, VEC>(u);
+          else if (store) store_once(qo + l * so, pack_lanes<T, VEC>(u));
           if constexpr (SHARED) {
             float e[VEC];
             from_lanes(d, e);
-            dgs[l] = 0.f;
+            float t = e[0];
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) dgs[l] += e[v];
+            for (int v = 1; v < VEC; ++v) t += e[v];
+            dgs[SHARED ? l : 0] = t;
           } else {
-            if (all.value || (live && l < left)) store_once(qdg + l * sdg, pack_lanes<TG, VEC>(d));
+            if constexpr (tile_out.value) *g_at(l) = pack_lanes<TG, VEC>(d);
+            else if (store) store_once(qdg + l * sdg, pack_lanes<TG, VEC>(d));
           }
         }
-      };
-      if (full && left > L) walk(std::true_type{}); else walk(std::false_type{});
-      if constexpr (SHARED) {
-        // Sum each token's terms over the head: the first rounds halve the tokens a lane
-        // holds while they halve the lanes, so L sums cost about L + 5 shuffles.
+      }
+    };
+    if constexpr (RING) {
+      if (n == L && !(BWD && last_run)) {
+        walk(std::true_type{}, std::true_type{});
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          const int r = (int)(down ? row0 - i0 - (L - 1) : row0 + i0), x0 = tile * TILE;
+          uint8_t* from = ring + stage * BYTES;
+          tma_store_3d(&maps.out, from, x0, r, (int)b);
+          if (BWD && !SHARED) tma_store_3d(&maps.dg, from + 2 * L * PX, x0, r, (int)b);
+          bulk_commit_group();
+        }
+      } else if (n > 0) {
+        walk(std::false_type{}, std::false_type{});
+      }
+    } else {
+      if (whole && n == L && !(BWD && last_run)) walk(std::true_type{}, std::false_type{});
+      else walk(std::false_type{}, std::false_type{});
+    }
+    if constexpr (BWD && SHARED) {
+      // Sum each token's terms over the head: the first rounds halve the tokens a lane
+      // holds while they halve the lanes, so L sums cost about L + 5 shuffles.
+      if (n > 0) {
         int off = 16;
 #pragma unroll
-        for (int n = L; n > 1; n >>= 1, off >>= 1) {
+        for (int m = L; m > 1; m >>= 1, off >>= 1) {
           const bool up = lane & off;
 #pragma unroll
-          for (int j = 0; j < n / 2; ++j) {
-            const float send = up ? dgs[j] : dgs[j + n / 2], keep = up ? dgs[j + n / 2] : dgs[j];
-            dgs[j] = keep + __shfl_xor_sync(0xffffffffu, send, off);
+          for (int j = 0; j < m / 2; ++j) {
+            const float give = up ? dgs[j] : dgs[j + m / 2], keep = up ? dgs[j + m / 2] : dgs[j];
+            dgs[j] = keep + __shfl_xor_sync(0xffffffffu, give, off);
           }
         }
         float total = dgs[0];
         const int per = 2 * off;                     // lanes that hold parts of one token
         for (; off; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-        if (lane % per == 0 && lane / per < left) qdg[lane / per * sdg] = from_f32<TG>(total);
+        if (lane % per == 0 && lane / per < n) qdg[lane / per * sdg] = from_f32<TG>(total);
       }
     }
+    if (++stage == kStages) {
+      stage = 0;
+      full_phase ^= 1;
+    }
+  }
+  if (RING && lane == 0) {
+    if (given_up) {                                  // copies that were issued land before the CTA exits
+      const uint64_t t0 = globaltimer();
+      for (int s = 0; s < kStages && i0 < len; ++s, i0 += round_tokens) {
+        while (!mbar_try_wait(&full[warp][stage], full_phase) && globaltimer() - t0 < kWaitLimitNs) {
+        }
+        if (++stage == kStages) {
+          stage = 0;
+          full_phase ^= 1;
+        }
+      }
+    }
+    bulk_wait_group<0>();                            // results are written before the CTA exits
   }
   if (given_up && threadIdx.x == 0 && p.status) atomicExch(p.status, VDN_ERR_TIMEOUT);
   if (p.last && rank == 0 && warp == 0 && live) {
@@ -417,6 +539,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 5) scan_kernel(const Params p,
 #pragma unroll
     for (int v = 0; v < VEC; ++v) p.last[seq * p.channels + c + v] = e[v];
   }
+  __syncwarp();
+  cluster_sync();                                    // nobody leaves while lines may still be sent to it
 }
 
 // One token per sequence (serving): h = a h + x, one thread per VEC channels.
@@ -445,10 +569,114 @@ __global__ void __launch_bounds__(256) step_kernel(const Params p, const int hea
   }
 }
 
-static int pow2_at_least(int64_t n, int most) {
+template <int MOST>
+static int pow2_at_least(int64_t n) {                // the least power of two >= n, at most MOST
+  static_assert(MOST > 0 && (MOST & (MOST - 1)) == 0, "a power of two bounds a power of two");
   int v = 1;
-  while (v < n && v < most) v *= 2;
+  while (v < n && v < MOST) v *= 2;
   return v;
+}
+
+template <typename T>
+static CUtensorMapDataType map_type() {
+  return sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+         : std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+// Boxes of `tokens` rows x `tile` channels over [batches, rows, channels].
+template <typename T>
+static int rows_map(CUtensorMap* map, const void* base, int64_t channels, int64_t rows, int64_t batches, int64_t row,
+                    int64_t batch, int tile, int tokens) {
+  const int64_t one = (channels * (int64_t)sizeof(T) + 15) / 16 * 16;   // a stride that no index multiplies
+  cuuint64_t dims[3] = {(cuuint64_t)channels, (cuuint64_t)rows, (cuuint64_t)batches};
+  cuuint64_t strides[2] = {(cuuint64_t)(row ? row * (int64_t)sizeof(T) : one),
+                           (cuuint64_t)(batch ? batch * (int64_t)sizeof(T) : one)};
+  cuuint32_t box[3] = {(cuuint32_t)tile, (cuuint32_t)tokens, 1};
+  return encode_map_swizzle(map, map_type<T>(), 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+template <typename T>
+static bool map_takes(const void* base, int64_t rows, int64_t batches, int64_t row, int64_t batch) {
+  return aligned16(base) && row * (int64_t)sizeof(T) % 16 == 0 && batch * (int64_t)sizeof(T) % 16 == 0 &&
+         (rows == 1 || row > 0) && (batches == 1 || batch > 0);
+}
+
+constexpr int kDevices = 64;
+
+// Raises the kernel's shared-memory limit, once per device.
+template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED, int FROM>
+static int prepare(int& dev) {
+  constexpr int bytes = FROM == ROWS_LOAD ? 0 : kStages * tile_bytes<T, TG, VEC, L, BWD, SHARED>();
+  static bool set[kDevices] = {};
+  VDN_CUDA_TRY(cudaGetDevice(&dev));
+  VDN_CHECK_ARG(dev >= 0 && dev < kDevices, "device index out of range");
+  if (bytes && !set[dev]) {
+    VDN_CUDA_TRY(cudaFuncSetAttribute(scan_kernel<T, TG, VEC, L, BWD, SHARED, FROM>,
+                                      cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_WARPS * bytes));
+    set[dev] = true;
+  }
+  return VDN_OK;
+}
+
+template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED, int FROM>
+static void configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, int64_t blocks, int warps, int cluster) {
+  constexpr int bytes = FROM == ROWS_LOAD ? 0 : kStages * tile_bytes<T, TG, VEC, L, BWD, SHARED>();
+  cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(warps * 32);
+  cfg.dynamicSmemBytes = warps * bytes;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+}
+
+// CTAs that share a sequence.  More of them shorten the walk, but a grid that does not fit the
+// GPU at once runs in waves, and the last may be nearly empty (the clip's 80 tiles: 305 us
+// with 8 CTAs each, which needs 640 places where there are 592).  Time is taken as waves x rounds x the
+// longer of a round's latency (about three CTAs' work) and the work of the CTAs on an SM.
+// The ring kernel's places decide for both kernels, so the sums' order does not hang on alignment.
+template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED>
+static int choose_cluster(int64_t len, int64_t ids, int warps, int& cluster) {
+  constexpr int FROM = VEC > 1 || SHARED ? ROWS_UP : ROWS_LOAD;
+  static int places[kDevices][3][MAX_CLUSTER + 1] = {};
+  int dev = 0;
+  if (int rc = prepare<T, TG, VEC, L, BWD, SHARED, FROM>(dev)) return rc;
+  const int64_t runs = (len + warps * L - 1) / (warps * L);
+  cluster = 1;
+  double best = 0;
+  for (int c = 1; c <= MAX_CLUSTER && c <= (runs > 1 ? runs : 1); ++c) {
+    int& fit = places[dev][warps >> 1][c];           // clusters resident at once; warps is 1, 2 or 4
+    if (!fit) {
+      cudaLaunchConfig_t cfg;
+      cudaLaunchAttribute attr[1];
+      configure<T, TG, VEC, L, BWD, SHARED, FROM>(cfg, attr, 148 * 64 / c * c, warps, c);
+      int n = 0;
+      VDN_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, scan_kernel<T, TG, VEC, L, BWD, SHARED, FROM>, &cfg));
+      fit = n > 0 ? n : 1;
+    }
+    const int64_t waves = (ids + fit - 1) / fit, tail = ids - (waves - 1) * fit;
+    auto load = [&](int64_t clusters) { return clusters * c / 148.0 > 3 ? clusters * c / 148.0 : 3.0; };
+    const double t = (double)((runs + c - 1) / c) * ((waves - 1) * load(fit) + load(tail));
+    if (c == 1 || t < best) {
+      best = t;
+      cluster = c;
+    }
+  }
+  return VDN_OK;
+}
+
+template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED, int FROM>
+static int launch_from(const Params& p, int warps, int cluster, const Maps& maps, cudaStream_t stream) {
+  const int64_t ids = (p.seqs + (p.zero_tail ? 1 : 0)) * p.tiles;
+  VDN_CHECK_ARG(ids * cluster < (1ll << 31), "too many sequences times channels for one launch");
+  int dev = 0;
+  if (int rc = prepare<T, TG, VEC, L, BWD, SHARED, FROM>(dev)) return rc;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[1];
+  configure<T, TG, VEC, L, BWD, SHARED, FROM>(cfg, attr, ids * cluster, warps, cluster);
+  cfg.stream = stream;
+  VDN_CUDA_TRY(cudaLaunchKernelEx(&cfg, scan_kernel<T, TG, VEC, L, BWD, SHARED, FROM>, p, cluster, maps));
+  return VDN_OK;
 }
 
 template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED>
@@ -456,22 +684,33 @@ static int launch(const Params& p, cudaStream_t stream) {
   // The typical length decides how many warps and CTAs share a sequence (a packed batch's
   // lengths live on the device: their mean stands for them).
   const int64_t len = p.cu ? (p.rows + p.seqs - 1) / p.seqs : (int64_t)p.rows;
-  const int warps = pow2_at_least((len + L - 1) / L, MAX_WARPS);
-  const int cluster = pow2_at_least((len + warps * L - 1) / (warps * L), MAX_CLUSTER);
-  const int64_t ids = (p.seqs + (p.zero_tail ? 1 : 0)) * p.tiles;
-  VDN_CHECK_ARG(ids * cluster < (1ll << 31), "too many sequences times channels for one launch");
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(ids * cluster));
-  cfg.blockDim = dim3(warps * 32);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  VDN_CUDA_TRY(cudaLaunchKernelEx(&cfg, scan_kernel<T, TG, VEC, L, BWD, SHARED>, p, cluster));
-  return VDN_OK;
+  const int warps = pow2_at_least<MAX_WARPS>((len + L - 1) / L);
+  int cluster = 1;
+  if (int rc = choose_cluster<T, TG, VEC, L, BWD, SHARED>(len, p.seqs * p.tiles, warps, cluster)) return rc;
+  Maps maps = {};
+  // Tiles of whole runs pay from two runs a sequence on; shorter ones would mostly copy others' rows.
+  if constexpr (VEC > 1 || SHARED) {
+    const int64_t batches = p.cu ? 1 : p.seqs, rows = p.rows;
+    const bool ring = len >= 2 * L && map_takes<T>(p.x, rows, batches, p.x_row, p.x_batch) &&
+                      (SHARED || map_takes<TG>(p.g, rows, batches, p.g_row, p.g_batch)) &&
+                      map_takes<T>(p.out, rows, batches, p.out_row, p.out_batch) &&
+                      (!BWD || map_takes<T>(p.y_in, rows, batches, p.y_row, p.y_batch)) &&
+                      (!BWD || SHARED || map_takes<TG>(p.dg, rows, batches, p.dg_row, p.dg_batch));
+    if (ring) {
+      const int64_t c = p.channels;
+      if (int rc = rows_map<T>(&maps.x, p.x, c, rows, batches, p.x_row, p.x_batch, 32 * VEC, L)) return rc;
+      if (int rc = rows_map<T>(&maps.out, p.out, c, rows, batches, p.out_row, p.out_batch, 32 * VEC, L)) return rc;
+      if (!SHARED)
+        if (int rc = rows_map<TG>(&maps.g, p.g, c, rows, batches, p.g_row, p.g_batch, 32 * VEC, L)) return rc;
+      if (BWD)
+        if (int rc = rows_map<T>(&maps.y, p.y_in, c, rows, batches, p.y_row, p.y_batch, 32 * VEC, L)) return rc;
+      if (BWD && !SHARED)
+        if (int rc = rows_map<TG>(&maps.dg, p.dg, c, rows, batches, p.dg_row, p.dg_batch, 32 * VEC, L)) return rc;
+      if (p.reverse != BWD) return launch_from<T, TG, VEC, L, BWD, SHARED, ROWS_DOWN>(p, warps, cluster, maps, stream);
+      return launch_from<T, TG, VEC, L, BWD, SHARED, ROWS_UP>(p, warps, cluster, maps, stream);
+    }
+  }
+  return launch_from<T, TG, VEC, L, BWD, SHARED, ROWS_LOAD>(p, warps, cluster, maps, stream);
 }
 
 template <typename T, typename TG, bool BWD>
@@ -505,7 +744,7 @@ static int dispatch(Params& p, int shared_dim, cudaStream_t stream) {
   }
   // Tokens a warp: as many as its registers hold (the backward keeps twice the arrays),
   // the same whatever the alignment, so that strides do not change the order of the sums.
-  constexpr int L = BWD ? 8 : 16;
+  constexpr int L = 16;
   if (shared_dim) {                                  // one head per tile
     const int vec = shared_dim / 32;
     VDN_CHECK_ARG(fits(vec), "a shared decay needs rows aligned to %d elements", vec);
