@@ -15,7 +15,7 @@
 //   * a warp owns L tokens of 32 * VEC channels (lane = VEC neighbouring channels) and folds
 //     them into (A, H), keeping for each token its state from zero and its reach, the
 //     product of the decays so far; after the join its true states are state + reach * carry;
-//   * a CTA of up to four warps owns neighbouring runs, joined through shared memory;
+//   * a CTA of up to eight warps owns neighbouring runs, joined through shared memory;
 //   * a cluster of up to eight CTAs owns neighbouring CTA runs and walks the sequence in
 //     rounds.  Each CTA sends its pair into the others' shared memory with asynchronous
 //     stores that count on their mbarriers: unlike a cluster barrier (whose release waits
@@ -42,7 +42,10 @@ namespace gscan {
 
 using namespace sm100;
 
-constexpr int MAX_WARPS = 4, MAX_CLUSTER = 8;
+constexpr int MAX_CLUSTER = 8;
+// Warps a CTA, at most: the backward per channel keeps the most tiles, so that eight warps would
+// leave one CTA an SM (480 us against 327 on the clip).
+template <bool BWD, bool SHARED> constexpr int max_warps() { return BWD && !SHARED ? 4 : 8; }
 
 struct Params {
   const void* x;        // forward: x; backward: dy
@@ -70,9 +73,11 @@ __device__ __forceinline__ f2 two_to(f2 t) {
   f2_unpack(t, a, b);
   return f2_pack(two_to(a), two_to(b));
 }
-__device__ __forceinline__ float clamp_decay(float g) {       // NaN stays NaN
+// log decays as loaded, held in [-87.9, 88.75] (where two_to works); NaN stays NaN.  16-bit pairs
+// are clamped in one instruction before they are widened.
+__device__ __forceinline__ float clamp_decay(float g) {
   float r;
-  asm("max.NaN.f32 %0, %1, 0fC2AFCCCD;\n\tmin.NaN.f32 %0, %0, 0f42B18000;" : "=f"(r) : "f"(g));   // [-87.9, 88.75]
+  asm("max.NaN.f32 %0, %1, 0fC2AFCCCD;\n\tmin.NaN.f32 %0, %0, 0f42B18000;" : "=f"(r) : "f"(g));
   return r;
 }
 __device__ __forceinline__ f2 clamp_decay(f2 g) {
@@ -80,12 +85,41 @@ __device__ __forceinline__ f2 clamp_decay(f2 g) {
   f2_unpack(g, a, b);
   return f2_pack(clamp_decay(a), clamp_decay(b));
 }
+template <typename T> __device__ __forceinline__ uint32_t clamp_word(uint32_t w);
+template <> __device__ __forceinline__ uint32_t clamp_word<float>(uint32_t w) {
+  return __float_as_uint(clamp_decay(__uint_as_float(w)));
+}
+template <> __device__ __forceinline__ uint32_t clamp_word<__nv_bfloat16>(uint32_t w) {   // -88, 88.5
+  uint32_t r;
+  asm("{\n\t.reg .b32 t;\n\tmax.NaN.bf16x2 t, %1, %2;\n\tmin.NaN.bf16x2 %0, t, %3;\n\t}" : "=r"(r) : "r"(w), "r"(0xC2B0C2B0u), "r"(0x42B142B1u));
+  return r;
+}
+template <> __device__ __forceinline__ uint32_t clamp_word<__half>(uint32_t w) {          // -87.875, 88.5
+  uint32_t r;
+  asm("{\n\t.reg .b32 t;\n\tmax.NaN.f16x2 t, %1, %2;\n\tmin.NaN.f16x2 %0, t, %3;\n\t}" : "=r"(r) : "r"(w), "r"(0xD57ED57Eu), "r"(0x55885588u));
+  return r;
+}
+template <typename TG, int GV, typename V, int N>
+__device__ __forceinline__ void unpack_decays(const Raw<TG, GV>& raw, V (&g)[N]) {
+  if constexpr (GV * sizeof(TG) < 4) {
+    float e[1];
+    unpack<TG, 1>(raw, e);
+    e[0] = clamp_decay(e[0]);
+    to_lanes(e, g);
+  } else {
+    uint32_t w[GV * sizeof(TG) / 4];
+    words(raw, w);
+#pragma unroll
+    for (auto& x : w) x = clamp_word<TG>(x);
+    const auto held = join(w);
+    unpack_lanes<TG, GV>(held, g);
+  }
+}
 
-// exp(g) as hi + lo (see above): n = round(g / ln 2), r = g - n ln 2, e = expm1(r).
+// exp(g) as hi + lo (see above), g clamped: n = round(g / ln 2), r = g - n ln 2, e = expm1(r).
 template <typename V>
 __device__ __forceinline__ void decay_pair(V g, V& hi, V& lo) {
   auto c = [](float v) { return vset(V{}, v); };
-  g = clamp_decay(g);
   const V t = vfma(g, c(1.4426950408889634f), c(12582912.0f + 127.0f));
   const V n = vadd(t, c(-12582912.0f - 127.0f));
   V r = vfma(n, c(-0.693359375f), g);                // exact: n has 8 bits, the constant 12
@@ -100,9 +134,9 @@ __device__ __forceinline__ void decay_pair(V g, V& hi, V& lo) {
   lo = vmul(vadd(e, vfma(one, c(-1.0f), c(1.0f))), scale);
 }
 template <typename V>
-__device__ __forceinline__ V decay_of(V g) {
+__device__ __forceinline__ V decay_of(V g) {         // of any g
   V hi, lo;
-  decay_pair(g, hi, lo);
+  decay_pair(clamp_decay(g), hi, lo);
   return vadd(hi, lo);
 }
 
@@ -136,10 +170,10 @@ constexpr int tile_bytes() {   // of one warp and stage: x (dy), the saved y, th
 }
 
 template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED, int FROM>
-__global__ void __launch_bounds__(MAX_WARPS * 32, FROM == ROWS_LOAD ? 3 : 4)
+__global__ void __launch_bounds__(max_warps<BWD, SHARED>() * 32, BWD && !SHARED ? 3 : 2)
     scan_kernel(const Params p, const int cluster, const __grid_constant__ Maps maps) {
   constexpr int GV = SHARED ? 1 : VEC;               // decays per lane and token
-  constexpr int TILE = 32 * VEC;
+  constexpr int TILE = 32 * VEC, MAX_WARPS = max_warps<BWD, SHARED>();
   constexpr bool RING = FROM != ROWS_LOAD;
   using RX = Raw<T, VEC>;
   using RG = Raw<TG, GV>;
@@ -254,7 +288,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, FROM == ROWS_LOAD ? 3 : 4)
     const bool in = lane < L && i + lane < len;
     float e[1] = {0.f};
     if (in) unpack<TG, 1>(*reinterpret_cast<const Raw<TG, 1>*>(pg + (i + lane) * sg), e);
-    return e[0];
+    return clamp_decay(e[0]);
   };
   float g_next = SHARED ? load_shared(i0) : 0.f;
 
@@ -316,7 +350,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, FROM == ROWS_LOAD ? 3 : 4)
           hi[0] = vset(G{}, __shfl_sync(0xffffffffu, hi_lane, l));
           lo[0] = vset(G{}, __shfl_sync(0xffffffffu, lo_lane, l));
         } else {
-          unpack_lanes<TG, GV>(RING ? *g_at(l) : rg[RING || SHARED ? 0 : l], g);
+          unpack_decays<TG, GV>(RING ? *g_at(l) : rg[RING || SHARED ? 0 : l], g);
         }
 #pragma unroll
         for (int v = 0; v < NG; ++v) {
@@ -348,22 +382,17 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, FROM == ROWS_LOAD ? 3 : 4)
     }
 
     // Join the warps of the CTA: `before` is the fold of the warps in front of this one.
+    // (Inside a round the product of the run's decays will do; the sums carry the long chain.)
     Fold<V> own[NV], before[NV];
-    {
-      G a[NG];
 #pragma unroll
-      for (int v = 0; v < NG; ++v) {
-        a[v] = decay_of(sum[v]);
-        sums[buf][warp][v][lane] = sum[v];
-      }
+    for (int v = 0; v < NG; ++v) sums[buf][warp][v][lane] = sum[v];
 #pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        spread(a[SHARED ? 0 : v], own[v].a);
-        own[v].h = fold[v];
-        folds[buf][warp][v][lane] = own[v];
-        before[v].a = vset(V{}, 1.f);
-        before[v].h = vset(V{}, 0.f);
-      }
+    for (int v = 0; v < NV; ++v) {
+      spread(far[SHARED ? 0 : v], own[v].a);
+      own[v].h = fold[v];
+      folds[buf][warp][v][lane] = own[v];
+      before[v].a = vset(V{}, 1.f);
+      before[v].h = vset(V{}, 0.f);
     }
     if (!__syncthreads_and(ok && !given_up)) break;  // a wait that gave up ends the whole CTA
 #pragma unroll
@@ -402,21 +431,16 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, FROM == ROWS_LOAD ? 3 : 4)
     mbar_wait(&arrived[buf], phase, &given_up);      // a failure ends the loop at the next round's barrier
     phase ^= buf;
     V in[NV];                                        // the true carry in front of this warp
+    const Fold<V>(*line)[NV][32] = &runs[buf][0];
+    auto pass = [&](int from, int to) {
+      for (int r = from; r < to; ++r)
 #pragma unroll
-    for (int v = 0; v < NV; ++v) in[v] = carry[v];
+        for (int v = 0; v < NV; ++v) carry[v] = vfma(line[r][v][lane].a, carry[v], line[r][v][lane].h);
+    };
+    pass(0, rank);
 #pragma unroll
-    for (int r = 0; r < MAX_CLUSTER; ++r) {
-      if (r < cluster) {
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-          if (r == rank) in[v] = carry[v];
-          const Fold<V> f = runs[buf][r][v][lane];
-          carry[v] = vfma(f.a, carry[v], f.h);
-        }
-      }
-    }
-#pragma unroll
-    for (int v = 0; v < NV; ++v) in[v] = vfma(before[v].a, in[v], before[v].h);
+    for (int v = 0; v < NV; ++v) in[v] = vfma(before[v].a, carry[v], before[v].h);
+    pass(rank, cluster);
 
     // Second walk, with the true carry.  A whole run of a ring takes the place of its inputs
     // and leaves as it came; others are stored row by row.
@@ -558,7 +582,7 @@ __global__ void __launch_bounds__(256) step_kernel(const Params p, const int hea
 #pragma unroll
   for (int v = 0; v < VEC; ++v) {
     float hi, lo;
-    decay_pair(g[SHARED ? 0 : v], hi, lo);
+    decay_pair(clamp_decay(g[SHARED ? 0 : v]), hi, lo);
     h[v] = p.first ? p.first[seq * p.channels + c + v] : 0.f;
     h[v] = fmaf(hi, h[v], fmaf(lo, h[v], x[v]));
   }
@@ -610,7 +634,7 @@ static int prepare(int& dev) {
   VDN_CHECK_ARG(dev >= 0 && dev < kDevices, "device index out of range");
   if (bytes && !set[dev]) {
     VDN_CUDA_TRY(cudaFuncSetAttribute(scan_kernel<T, TG, VEC, L, BWD, SHARED, FROM>,
-                                      cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_WARPS * bytes));
+                                      cudaFuncAttributeMaxDynamicSharedMemorySize, max_warps<BWD, SHARED>() * bytes));
     set[dev] = true;
   }
   return VDN_OK;
@@ -630,36 +654,44 @@ static void configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, int64_
   cfg.numAttrs = 1;
 }
 
-// CTAs that share a sequence.  More of them shorten the walk, but a grid that does not fit the
-// GPU at once runs in waves, and the last may be nearly empty (the clip's 80 tiles: 305 us
-// with 8 CTAs each, which needs 640 places where there are 592).  Time is taken as waves x rounds x the
-// longer of a round's latency (about three CTAs' work) and the work of the CTAs on an SM.
-// The ring kernel's places decide for both kernels, so the sums' order does not hang on alignment.
+// Warps a CTA and CTAs a cluster.  More CTAs on a sequence shorten its walk, but a grid that does
+// not fit the GPU at once runs in waves, the last perhaps nearly empty (the clip's 80 tiles:
+// 305 us with clusters of 8, which need 640 places where there are 592, and 282 us with 5),
+// and every CTA starts up anew.  Measured over clusters of one to eight, CTAs of four and
+// eight warps and nine shapes, a round takes about as long as 1 + (the warps on the fullest SM)
+// / 4, and starting up as two rounds; choosing by that was within a tenth of the best of
+// them.  The ring kernel's places decide for both kernels, so that the order of the sums does
+// not hang on alignment.
 template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED>
-static int choose_cluster(int64_t len, int64_t ids, int warps, int& cluster) {
-  constexpr int FROM = VEC > 1 || SHARED ? ROWS_UP : ROWS_LOAD;
-  static int places[kDevices][3][MAX_CLUSTER + 1] = {};
+static int choose_shape(int64_t len, int64_t ids, int& warps, int& cluster) {
+  constexpr int FROM = VEC > 1 || SHARED ? ROWS_UP : ROWS_LOAD, MAX_WARPS = max_warps<BWD, SHARED>();
+  static int places[kDevices][4][MAX_CLUSTER + 1] = {};
   int dev = 0;
   if (int rc = prepare<T, TG, VEC, L, BWD, SHARED, FROM>(dev)) return rc;
-  const int64_t runs = (len + warps * L - 1) / (warps * L);
+  warps = pow2_at_least<MAX_WARPS>((len + L - 1) / L);
   cluster = 1;
-  double best = 0;
-  for (int c = 1; c <= MAX_CLUSTER && c <= (runs > 1 ? runs : 1); ++c) {
-    int& fit = places[dev][warps >> 1][c];           // clusters resident at once; warps is 1, 2 or 4
-    if (!fit) {
-      cudaLaunchConfig_t cfg;
-      cudaLaunchAttribute attr[1];
-      configure<T, TG, VEC, L, BWD, SHARED, FROM>(cfg, attr, 148 * 64 / c * c, warps, c);
-      int n = 0;
-      VDN_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, scan_kernel<T, TG, VEC, L, BWD, SHARED, FROM>, &cfg));
-      fit = n > 0 ? n : 1;
-    }
-    const int64_t waves = (ids + fit - 1) / fit, tail = ids - (waves - 1) * fit;
-    auto load = [&](int64_t clusters) { return clusters * c / 148.0 > 3 ? clusters * c / 148.0 : 3.0; };
-    const double t = (double)((runs + c - 1) / c) * ((waves - 1) * load(fit) + load(tail));
-    if (c == 1 || t < best) {
-      best = t;
-      cluster = c;
+  int64_t best = -1;
+  const int most = warps;                            // fewer warps only from eight to four
+  for (int w = most; w == most || w >= 4; w /= 2) {
+    const int64_t runs = (len + w * L - 1) / (w * L);
+    for (int c = 1; c <= MAX_CLUSTER && c <= (runs > 1 ? runs : 1); ++c) {
+      int& fit = places[dev][w == 8 ? 3 : w >> 1][c];   // clusters resident at once
+      if (!fit) {
+        cudaLaunchConfig_t cfg;
+        cudaLaunchAttribute attr[1];
+        configure<T, TG, VEC, L, BWD, SHARED, FROM>(cfg, attr, 148 * 64 / c * c, w, c);
+        int n = 0;
+        VDN_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, scan_kernel<T, TG, VEC, L, BWD, SHARED, FROM>, &cfg));
+        fit = n > 0 ? n : 1;
+      }
+      const int64_t waves = (ids + fit - 1) / fit, tail = ids - (waves - 1) * fit;
+      auto load = [&](int64_t clusters) { return 4 + w * ((clusters * c + 147) / 148); };
+      const int64_t t = ((runs + c - 1) / c + 2) * ((waves - 1) * load(fit) + load(tail));
+      if (best < 0 || t < best) {
+        best = t;
+        warps = w;
+        cluster = c;
+      }
     }
   }
   return VDN_OK;
@@ -684,9 +716,8 @@ static int launch(const Params& p, cudaStream_t stream) {
   // The typical length decides how many warps and CTAs share a sequence (a packed batch's
   // lengths live on the device: their mean stands for them).
   const int64_t len = p.cu ? (p.rows + p.seqs - 1) / p.seqs : (int64_t)p.rows;
-  const int warps = pow2_at_least<MAX_WARPS>((len + L - 1) / L);
-  int cluster = 1;
-  if (int rc = choose_cluster<T, TG, VEC, L, BWD, SHARED>(len, p.seqs * p.tiles, warps, cluster)) return rc;
+  int warps = 1, cluster = 1;
+  if (int rc = choose_shape<T, TG, VEC, L, BWD, SHARED>(len, p.seqs * p.tiles, warps, cluster)) return rc;
   Maps maps = {};
   // Tiles of whole runs pay from two runs a sequence on; shorter ones would mostly copy others' rows.
   if constexpr (VEC > 1 || SHARED) {
