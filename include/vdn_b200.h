@@ -442,29 +442,31 @@ int vdn_layer_norm_backward(const void* dy, int dtype, int64_t rows, int64_t wid
 
 /* Linear layer on tcgen05, 16-bit operands (`dtype` bf16 or fp16, all matrices alike), fp32
  * accumulation: z = x w^T + bias, pre = z (if not NULL), y = act(z) + residual (if not
- * NULL).  x [rows, k] and w [n, k] 16-byte aligned with row strides multiples of 8
- * elements; bias [n], residual, y and pre [rows, n] with any row stride.  y must not
- * overlap the inputs.  act: VDN_ACT_NONE, _GELU_TANH, _GELU_ERF or _SILU.  status: as in
- * vdn_mxfp8_gemm.  The 16-bit, trainable counterpart of the block's MXFP8 projections with
- * fused epilogues (src/models/ops/mxfp8_linear.py:60-102). */
+ * NULL).  x [rows, k], w [n, k], bias [n], residual, y and pre [rows, n]; columns contiguous,
+ * row strides in elements.  x or w whose address or stride is not a multiple of 16 bytes is
+ * copied into the workspace first (vdn_linear_workspace_size; 0 and NULL otherwise).  y
+ * must not overlap the inputs.  act: VDN_ACT_NONE, _GELU_TANH, _GELU_ERF or _SILU.  status:
+ * as in vdn_mxfp8_gemm.  The 16-bit, trainable counterpart of the block's MXFP8
+ * projections with fused epilogues (src/models/ops/mxfp8_linear.py:60-102). */
+size_t vdn_linear_workspace_size(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows,
+                                 int64_t n, int64_t k);
 int vdn_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
                    const void* residual, int64_t ldr, int dtype, int act, int64_t rows, int64_t n,
-                   int64_t k, void* y, int64_t ldy, void* pre, int64_t ldp, int* status,
-                   cudaStream_t stream);
+                   int64_t k, void* y, int64_t ldy, void* pre, int64_t ldp, void* workspace,
+                   size_t workspace_bytes, int* status, cudaStream_t stream);
 
-/* dz = dy act'(pre) [rows, n] (nothing is written for VDN_ACT_NONE: dz is dy) and d_bias [n]
- * (or NULL) = its column sums, in fp32 and a fixed order through the workspace. */
-size_t vdn_linear_dz_workspace_size(int64_t rows, int64_t n);
-int vdn_linear_dz(const void* dy, int64_t ldy, const void* pre, int64_t ldp, int dtype, int act,
-                  int64_t rows, int64_t n, void* dz, int64_t ldz, void* d_bias, void* workspace,
-                  size_t workspace_bytes, cudaStream_t stream);
-
-/* dx [rows, k] = dz [rows, n] w [n, k], and dw [n, k] = dz^T x [rows, k].  dz, w and x as the
- * operands of vdn_linear_act, the outputs with any row stride. */
-int vdn_linear_dx(const void* dz, int64_t ldz, const void* w, int64_t ldw, int dtype, int64_t rows,
-                  int64_t n, int64_t k, void* dx, int64_t ldx, int* status, cudaStream_t stream);
-int vdn_linear_dw(const void* dz, int64_t ldz, const void* x, int64_t ldx, int dtype, int64_t rows,
-                  int64_t n, int64_t k, void* dw, int64_t ldw, int* status, cudaStream_t stream);
+/* Gradients of vdn_linear_act from dy and its `pre` (not read for VDN_ACT_NONE): with dz = dy
+ * act'(pre), dx = dz w, dw = dz^T x and d_bias = the column sums of dz, each left out when
+ * NULL.  dz is rounded to dtype for the two products; d_bias sums it unrounded, in fp32 and a
+ * fixed order.  The residual's gradient is dy. */
+size_t vdn_linear_backward_workspace_size(const void* dy, int64_t ldy, const void* x, int64_t ldx,
+                                          const void* w, int64_t ldw, int act, int64_t rows, int64_t n,
+                                          int64_t k);
+int vdn_linear_act_backward(const void* dy, int64_t ldy, const void* pre, int64_t ldp, const void* x,
+                            int64_t ldx, const void* w, int64_t ldw, int dtype, int act, int64_t rows,
+                            int64_t n, int64_t k, void* dx, int64_t lddx, void* dw, int64_t lddw,
+                            void* d_bias, void* workspace, size_t workspace_bytes, int* status,
+                            cudaStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -83,12 +83,12 @@ SIGNATURES = {
     "vdn_layer_norm_backward_workspace_size": (_sz, [_i64, _i64]),
     "vdn_layer_norm_backward": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _i32, _p, _p, _p, _i64, _p, _p,
                                        _p, _sz, _p, _p]),
+    "vdn_linear_workspace_size": (_sz, [_p, _i64, _p, _i64, _i64, _i64, _i64]),
     "vdn_linear_act": (_i32, [_p, _i64, _p, _i64, _p, _p, _i64, _i32, _i32, _i64, _i64, _i64, _p, _i64, _p, _i64,
-                              _p, _p]),
-    "vdn_linear_dz_workspace_size": (_sz, [_i64, _i64]),
-    "vdn_linear_dz": (_i32, [_p, _i64, _p, _i64, _i32, _i32, _i64, _i64, _p, _i64, _p, _p, _sz, _p]),
-    "vdn_linear_dx": (_i32, [_p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _p, _i64, _p, _p]),
-    "vdn_linear_dw": (_i32, [_p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _p, _i64, _p, _p]),
+                              _p, _sz, _p, _p]),
+    "vdn_linear_backward_workspace_size": (_sz, [_p, _i64, _p, _i64, _p, _i64, _i32, _i64, _i64, _i64]),
+    "vdn_linear_act_backward": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i32, _i32, _i64, _i64, _i64, _p,
+                                       _i64, _p, _i64, _p, _p, _sz, _p, _p]),
 }
 
 _LOCK = threading.Lock()

@@ -663,18 +663,19 @@ static void configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, int64_
 // them.  The ring kernel's places decide for both kernels, so that the order of the sums does
 // not hang on alignment.
 template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED>
-static int choose_shape(int64_t len, int64_t ids, int& warps, int& cluster) {
+static int choose_shape(int64_t mean, int64_t longest, int64_t seqs, int64_t tiles, int& warps, int& cluster) {
   constexpr int FROM = VEC > 1 || SHARED ? ROWS_UP : ROWS_LOAD, MAX_WARPS = max_warps<BWD, SHARED>();
   static int places[kDevices][4][MAX_CLUSTER + 1] = {};
   int dev = 0;
   if (int rc = prepare<T, TG, VEC, L, BWD, SHARED, FROM>(dev)) return rc;
-  warps = pow2_at_least<MAX_WARPS>((len + L - 1) / L);
+  warps = pow2_at_least<MAX_WARPS>((longest + L - 1) / L);
   cluster = 1;
+  const int64_t ids = seqs * tiles;
   int64_t best = -1;
   const int most = warps;                            // fewer warps only from eight to four
   for (int w = most; w == most || w >= 4; w /= 2) {
-    const int64_t runs = (len + w * L - 1) / (w * L);
-    for (int c = 1; c <= MAX_CLUSTER && c <= (runs > 1 ? runs : 1); ++c) {
+    const int64_t runs = (mean + w * L - 1) / (w * L), most_runs = (longest + w * L - 1) / (w * L);
+    for (int c = 1; c <= MAX_CLUSTER && c <= (most_runs > 1 ? most_runs : 1); ++c) {
       int& fit = places[dev][w == 8 ? 3 : w >> 1][c];   // clusters resident at once
       if (!fit) {
         cudaLaunchConfig_t cfg;
@@ -686,7 +687,9 @@ static int choose_shape(int64_t len, int64_t ids, int& warps, int& cluster) {
       }
       const int64_t waves = (ids + fit - 1) / fit, tail = ids - (waves - 1) * fit;
       auto load = [&](int64_t clusters) { return 4 + w * ((clusters * c + 147) / 148); };
-      const int64_t t = ((runs + c - 1) / c + 2) * ((waves - 1) * load(fit) + load(tail));
+      // the longest sequences' tiles go on alone
+      const int64_t t = ((runs + c - 1) / c + 2) * ((waves - 1) * load(fit) + load(tail)) +
+                        ((most_runs + c - 1) / c - (runs + c - 1) / c) * load(tiles);
       if (best < 0 || t < best) {
         best = t;
         warps = w;
@@ -713,11 +716,16 @@ static int launch_from(const Params& p, int warps, int cluster, const Maps& maps
 
 template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED>
 static int launch(const Params& p, cudaStream_t stream) {
-  // The typical length decides how many warps and CTAs share a sequence (a packed batch's
-  // lengths live on the device: their mean stands for them).
+  // A packed batch's lengths live on the device.  Their mean stands for most of them, and random
+  // cuts make the longest about 1 + ln(sequences) times as long.
   const int64_t len = p.cu ? (p.rows + p.seqs - 1) / p.seqs : (int64_t)p.rows;
+  int64_t longest = len;
+  if (p.cu) {
+    for (int64_t s = p.seqs; s > 1; s /= 2) longest += len * 7 / 10;
+    if (longest > p.rows) longest = p.rows;
+  }
   int warps = 1, cluster = 1;
-  if (int rc = choose_shape<T, TG, VEC, L, BWD, SHARED>(len, p.seqs * p.tiles, warps, cluster)) return rc;
+  if (int rc = choose_shape<T, TG, VEC, L, BWD, SHARED>(len, longest, p.seqs, p.tiles, warps, cluster)) return rc;
   Maps maps = {};
   // Tiles of whole runs pay from two runs a sequence on; shorter ones would mostly copy others' rows.
   if constexpr (VEC > 1 || SHARED) {

@@ -22,6 +22,8 @@
 // Rounding: z is rounded once for `pre` and once, after activation and residual in fp32,
 // for y.  dz is rounded to the operand type because the tensor cores take 16 bits; db sums
 // the unrounded dz.  Every wait is bounded (VDN_ERR_TIMEOUT).  No TMA multicast.
+#include <initializer_list>
+
 #include "train_common.cuh"
 #include "sm100.cuh"
 #include "tma_host.cuh"
@@ -807,18 +809,68 @@ static int product(const Operand& x, const Operand& f, int64_t depth, Params p, 
   return run_narrow<T, F_MN, X_MN, ACT, 128>(x, f, depth, p, d, stream);
 }
 
+// Copies up to two matrices into rows whose stride the tensor maps take (odd depths, unaligned views).
+struct Pad {
+  const uint16_t* src[2];
+  uint16_t* dst[2];
+  int64_t rows[2], cols[2], ld[2], to[2];
+};
+__global__ void __launch_bounds__(256) pad_kernel(const Pad p) {
+  const int m = blockIdx.y;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= p.rows[m]) return;
+  const uint16_t* s = p.src[m] + row * p.ld[m];
+  uint16_t* d = p.dst[m] + row * p.to[m];
+#pragma unroll 4
+  for (int64_t c = threadIdx.x & 31; c < p.cols[m]; c += 32) d[c] = s[c];
+}
+
+static int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+static bool fits_map(const void* base, int64_t ld, int64_t cols) { return aligned16(base) && ld >= cols && ld % 8 == 0; }
+static size_t padded_bytes(const void* base, int64_t ld, int64_t rows, int64_t cols) {
+  return fits_map(base, ld, cols) ? 0 : ((size_t)rows * pad8(cols) * 2 + 255) / 256 * 256;
+}
+
+// The operands as the tensor maps take them: as they lie, or copied into the workspace (which
+// advances past what was used).
+struct Matrix {
+  const void*& base;
+  int64_t& ld;
+  int64_t rows, cols;
+};
+static int settle(std::initializer_list<Matrix> operands, uint8_t*& ws, size_t& left, cudaStream_t stream) {
+  Pad p = {};
+  int n = 0;
+  int64_t most = 0;
+  for (const Matrix& o : operands) {
+    const size_t bytes = padded_bytes(o.base, o.ld, o.rows, o.cols);
+    if (!bytes) continue;
+    VDN_CHECK_ARG(ws && bytes <= left, "workspace smaller than the padded operands need");
+    p.src[n] = static_cast<const uint16_t*>(o.base);
+    p.dst[n] = reinterpret_cast<uint16_t*>(ws);
+    p.rows[n] = o.rows;
+    p.cols[n] = o.cols;
+    p.ld[n] = o.ld;
+    p.to[n] = pad8(o.cols);
+    most = o.rows > most ? o.rows : most;
+    o.base = ws;
+    o.ld = pad8(o.cols);
+    ws += bytes;
+    left -= bytes;
+    ++n;
+  }
+  if (!n) return VDN_OK;
+  pad_kernel<<<dim3((unsigned)((most + 7) / 8), n), 256, 0, stream>>>(p);
+  VDN_LAUNCH_CHECK("linear (padded operands)");
+  return VDN_OK;
+}
+
 static int check(int dtype, int64_t rows, int64_t n, int64_t k) {
   if (dtype != VDN_DTYPE_BF16 && dtype != VDN_DTYPE_F16) return set_error(VDN_ERR_TYPE, "linear takes bf16 or fp16");
   VDN_CHECK_ARG(rows >= 0 && n >= 1 && k >= 1, "bad linear extents");
   VDN_CHECK_ARG(rows < (1ll << 30) && n < (1ll << 30) && k < (1ll << 30), "extents too large");
   return VDN_OK;
 }
-static int check_operand(const void* base, int64_t ld, int64_t cols, const char* name) {
-  VDN_CHECK_ARG(base && aligned16(base) && ld >= cols && ld % 8 == 0,
-                "%s must be 16-byte aligned with a row stride that covers it and is a multiple of 8 elements", name);
-  return VDN_OK;
-}
-
 template <typename T, int ACT>
 static int forward(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t k, const Params& p, cudaStream_t s) {
   return product<T, false, false, ACT>({x, ldx, false}, {w, ldw, false}, k, p, s);
@@ -862,17 +914,25 @@ using namespace vdn;
     default: return set_error(VDN_ERR_VALUE, "unknown activation %d", act); \
   }
 
+extern "C" size_t vdn_linear_workspace_size(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows,
+                                            int64_t n, int64_t k) {
+  using namespace vdn::lact;
+  if (rows < 1 || n < 1 || k < 1) return 0;
+  return padded_bytes(x, ldx, rows, k) + padded_bytes(w, ldw, n, k);
+}
+
 extern "C" int vdn_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
                               const void* residual, int64_t ldr, int dtype, int act, int64_t rows, int64_t n,
-                              int64_t k, void* y, int64_t ldy, void* pre, int64_t ldp, int* status,
-                              cudaStream_t stream) {
+                              int64_t k, void* y, int64_t ldy, void* pre, int64_t ldp, void* workspace,
+                              size_t workspace_bytes, int* status, cudaStream_t stream) {
   using namespace vdn::lact;
   if (int rc = check(dtype, rows, n, k)) return rc;
+  VDN_CHECK_ARG(act == NONE || act == TANH || act == ERF || act == SILU, "unknown activation %d", act);
   if (rows == 0) return VDN_OK;
-  if (int rc = check_operand(x, ldx, k, "x")) return rc;
-  if (int rc = check_operand(w, ldw, k, "w")) return rc;
-  VDN_CHECK_ARG(y && ldy >= n && (!pre || ldp >= n) && (!residual || ldr >= 0), "bad output or residual");
+  VDN_CHECK_ARG(x && w && y && ldy >= n && (!pre || ldp >= n), "null pointer or bad row stride");
   VDN_CHECK_ARG(residual != y && (!pre || (pre != y && pre != residual)), "y, pre and residual must not overlap");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (int rc = settle({{x, ldx, rows, k}, {w, ldw, n, k}}, ws, workspace_bytes, stream)) return rc;
   Params p = {};
   p.bias = bias;
   p.resid = residual;
@@ -891,65 +951,102 @@ extern "C" int vdn_linear_act(const void* x, int64_t ldx, const void* w, int64_t
   }
 }
 
-extern "C" size_t vdn_linear_dz_workspace_size(int64_t rows, int64_t n) {
-  return rows < 1 || n < 1 ? 0 : sizeof(float) * (size_t)vdn::lact::kChunks * (size_t)n;
+namespace vdn {
+namespace lact {
+
+// What the backward needs beside its outputs: dz (or dy) where the tensor maps cannot read dy
+// itself, the bias gradient's partial sums, and x and w padded.
+static size_t dz_bytes(const void* dy, int64_t ldy, int act, int64_t rows, int64_t n) {
+  return act != NONE ? ((size_t)rows * pad8(n) * 2 + 255) / 256 * 256 : padded_bytes(dy, ldy, rows, n);
+}
+static size_t part_bytes(int64_t n) { return (sizeof(float) * kChunks * (size_t)n + 255) / 256 * 256; }
+
+template <typename T>
+static int backward(const void* dy, int64_t ldy, const void* pre, int64_t ldp, const void* x, int64_t ldx,
+                    const void* w, int64_t ldw, int act, int64_t rows, int64_t n, int64_t k, void* dx, int64_t lddx,
+                    void* dw, int64_t lddw, void* db, uint8_t* ws, size_t left, int* status, cudaStream_t stream) {
+  auto take = [&](size_t bytes) -> uint8_t* {
+    if (!ws || bytes > left) return nullptr;
+    uint8_t* at = ws;
+    ws += bytes;
+    left -= bytes;
+    return at;
+  };
+  float* part = nullptr;
+  if (db) {
+    part = reinterpret_cast<float*>(take(part_bytes(n)));
+    VDN_CHECK_ARG(part, "workspace smaller than vdn_linear_backward_workspace_size");
+  }
+  const void* dz = dy;
+  int64_t ldz = ldy;
+  void* out = nullptr;
+  if (act != NONE) {
+    out = take(dz_bytes(dy, ldy, act, rows, n));
+    VDN_CHECK_ARG(out, "workspace smaller than vdn_linear_backward_workspace_size");
+    dz = out;
+    ldz = pad8(n);
+  }
+  int rc = VDN_OK;
+  switch (act) {
+    case TANH: rc = dz_run<T, TANH>(dy, ldy, pre, ldp, out, ldz, rows, n, db, part, stream); break;
+    case ERF: rc = dz_run<T, ERF>(dy, ldy, pre, ldp, out, ldz, rows, n, db, part, stream); break;
+    case SILU: rc = dz_run<T, SILU>(dy, ldy, pre, ldp, out, ldz, rows, n, db, part, stream); break;
+    default: rc = dz_run<T, NONE>(dy, ldy, pre, ldp, nullptr, ldz, rows, n, db, part, stream);
+  }
+  if (rc) return rc;
+  if (dx) {
+    if (int rc2 = settle({{dz, ldz, rows, n}, {w, ldw, n, k}}, ws, left, stream)) return rc2;
+    Params p = {};
+    p.y = dx;
+    p.ldy = lddx;
+    p.rows = rows;
+    p.cols = k;
+    p.status = status;
+    if (int rc2 = product<T, false, true, NONE>({dz, ldz, false}, {w, ldw, true}, n, p, stream)) return rc2;
+  }
+  if (dw) {
+    if (int rc2 = settle({{dz, ldz, rows, n}, {x, ldx, rows, k}}, ws, left, stream)) return rc2;
+    Params p = {};
+    p.y = dw;
+    p.ldy = lddw;
+    p.rows = n;
+    p.cols = k;
+    p.status = status;
+    if (int rc2 = product<T, true, true, NONE>({dz, ldz, true}, {x, ldx, true}, rows, p, stream)) return rc2;
+  }
+  return VDN_OK;
 }
 
-extern "C" int vdn_linear_dz(const void* dy, int64_t ldy, const void* pre, int64_t ldp, int dtype, int act,
-                             int64_t rows, int64_t n, void* dz, int64_t ldz, void* d_bias, void* workspace,
-                             size_t workspace_bytes, cudaStream_t stream) {
+}  // namespace lact
+}  // namespace vdn
+
+extern "C" size_t vdn_linear_backward_workspace_size(const void* dy, int64_t ldy, const void* x, int64_t ldx,
+                                                     const void* w, int64_t ldw, int act, int64_t rows, int64_t n,
+                                                     int64_t k) {
   using namespace vdn::lact;
-  if (int rc = check(dtype, rows, n, 1)) return rc;
+  if (rows < 1 || n < 1 || k < 1) return 0;
+  return part_bytes(n) + dz_bytes(dy, ldy, act, rows, n) + padded_bytes(x, ldx, rows, k) + padded_bytes(w, ldw, n, k);
+}
+
+extern "C" int vdn_linear_act_backward(const void* dy, int64_t ldy, const void* pre, int64_t ldp, const void* x,
+                                       int64_t ldx, const void* w, int64_t ldw, int dtype, int act, int64_t rows,
+                                       int64_t n, int64_t k, void* dx, int64_t lddx, void* dw, int64_t lddw,
+                                       void* d_bias, void* workspace, size_t workspace_bytes, int* status,
+                                       cudaStream_t stream) {
+  using namespace vdn::lact;
+  if (int rc = check(dtype, rows, n, k)) return rc;
+  VDN_CHECK_ARG(act == NONE || act == TANH || act == ERF || act == SILU, "unknown activation %d", act);
+  VDN_CHECK_ARG((!dx || lddx >= k) && (!dw || lddw >= k), "bad output row stride");
   if (rows == 0) {
+    if (dw) VDN_CUDA_TRY(cudaMemset2DAsync(dw, (size_t)lddw * 2, 0, (size_t)k * 2, (size_t)n, stream));
     if (d_bias) VDN_CUDA_TRY(cudaMemsetAsync(d_bias, 0, (size_t)n * 2, stream));
     return VDN_OK;
   }
-  VDN_CHECK_ARG(dy && (act == VDN_ACT_NONE || (pre && dz && ldp >= 0 && ldz >= n)), "null pointer or bad row stride");
-  VDN_CHECK_ARG(!d_bias || (workspace && workspace_bytes >= vdn_linear_dz_workspace_size(rows, n)),
-                "workspace smaller than vdn_linear_dz_workspace_size");
-  float* part = static_cast<float*>(workspace);
-  if (dtype == VDN_DTYPE_BF16) {
-    VDN_LACT_BY_ACT(__nv_bfloat16, dz_run, dy, ldy, pre, ldp, dz, ldz, rows, n, d_bias, part, stream)
-  } else {
-    VDN_LACT_BY_ACT(__half, dz_run, dy, ldy, pre, ldp, dz, ldz, rows, n, d_bias, part, stream)
-  }
-}
-
-extern "C" int vdn_linear_dx(const void* dz, int64_t ldz, const void* w, int64_t ldw, int dtype, int64_t rows,
-                             int64_t n, int64_t k, void* dx, int64_t ldx, int* status, cudaStream_t stream) {
-  using namespace vdn::lact;
-  if (int rc = check(dtype, rows, n, k)) return rc;
-  if (rows == 0) return VDN_OK;
-  if (int rc = check_operand(dz, ldz, n, "dz")) return rc;
-  if (int rc = check_operand(w, ldw, k, "w")) return rc;
-  VDN_CHECK_ARG(dx && ldx >= k, "bad output");
-  Params p = {};
-  p.y = dx;
-  p.ldy = ldx;
-  p.rows = rows;
-  p.cols = k;
-  p.status = status;
-  if (dtype == VDN_DTYPE_BF16) return product<__nv_bfloat16, false, true, NONE>({dz, ldz, false}, {w, ldw, true}, n, p, stream);
-  return product<__half, false, true, NONE>({dz, ldz, false}, {w, ldw, true}, n, p, stream);
-}
-
-extern "C" int vdn_linear_dw(const void* dz, int64_t ldz, const void* x, int64_t ldx, int dtype, int64_t rows,
-                             int64_t n, int64_t k, void* dw, int64_t ldw, int* status, cudaStream_t stream) {
-  using namespace vdn::lact;
-  if (int rc = check(dtype, rows, n, k)) return rc;
-  VDN_CHECK_ARG(dw && ldw >= k, "bad output");
-  if (rows == 0) {
-    VDN_CUDA_TRY(cudaMemset2DAsync(dw, (size_t)ldw * 2, 0, (size_t)k * 2, (size_t)n, stream));
-    return VDN_OK;
-  }
-  if (int rc = check_operand(dz, ldz, n, "dz")) return rc;
-  if (int rc = check_operand(x, ldx, k, "x")) return rc;
-  Params p = {};
-  p.y = dw;
-  p.ldy = ldw;
-  p.rows = n;
-  p.cols = k;
-  p.status = status;
-  if (dtype == VDN_DTYPE_BF16) return product<__nv_bfloat16, true, true, NONE>({dz, ldz, true}, {x, ldx, true}, rows, p, stream);
-  return product<__half, true, true, NONE>({dz, ldz, true}, {x, ldx, true}, rows, p, stream);
+  VDN_CHECK_ARG(dy && (act == NONE || pre) && (!dx || w) && (!dw || x), "null pointer");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (dtype == VDN_DTYPE_BF16)
+    return backward<__nv_bfloat16>(dy, ldy, pre, ldp, x, ldx, w, ldw, act, rows, n, k, dx, lddx, dw, lddw, d_bias, ws,
+                                   workspace_bytes, status, stream);
+  return backward<__half>(dy, ldy, pre, ldp, x, ldx, w, ldw, act, rows, n, k, dx, lddx, dw, lddw, d_bias, ws,
+                          workspace_bytes, status, stream);
 }

@@ -11,6 +11,8 @@ backward is public as layer_norm_backward (the form to capture into a CUDA graph
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -20,6 +22,11 @@ from .mxfp8_linear import _status
 __all__ = ["layer_norm", "layer_norm_backward"]
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_size(rows, width):
+    return _lib.load().vdn_layer_norm_backward_workspace_size(rows, width)
 
 
 def _rows(t):
@@ -115,7 +122,7 @@ def _backward(grad_y, x, weight, mean, rstd, want_w, want_b, bias_dtype=None):
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     dw = torch.empty(width, dtype=kind, device=x.device) if want_w else None
     db = torch.empty(width, dtype=kind, device=x.device) if want_b else None
-    need = _lib.load().vdn_layer_norm_backward_workspace_size(rows, width)
+    need = _workspace_size(rows, width)
     ws = torch.empty(need, dtype=torch.uint8, device=x.device)
     w = None if weight is None else weight.contiguous()
     mean, rstd = mean.contiguous(), rstd.contiguous()

@@ -24,31 +24,20 @@ ACTIVATIONS = {"none": _lib.ACT_NONE, "gelu_tanh": _lib.ACT_GELU_TANH, "gelu_erf
                "silu": _lib.ACT_SILU}
 
 
-def _pad8(n):
-    return (n + 7) // 8 * 8
-
-
-def _operand(t, cols):
-    """t [..., cols] as the tensor maps take it: (rows of unit column stride, each 16-byte
-    aligned; their count; their stride), copied into padded rows where its layout does not suit them."""
-    if t.is_contiguous() and cols % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t, t.numel() // cols, cols
-    flat = t.reshape(-1, cols)
-    ld = flat.stride(0)
-    if flat.stride(1) != 1 or ld % 8 or ld < cols or flat.data_ptr() % 16:
-        ld = _pad8(cols)
-        flat = torch.empty(flat.shape[0], ld, dtype=t.dtype, device=t.device)[:, :cols].copy_(flat)
-    return flat, flat.shape[0], ld
-
-
 def _matrix(t, cols):
     """t [..., cols] as (rows of unit column stride, their count, their stride)."""
     if t.is_contiguous():
         return t, t.numel() // cols, cols
     flat = t.reshape(-1, cols)
-    if flat.stride(1) != 1 and cols != 1:
-        flat = flat.contiguous()
-    return flat, flat.shape[0], flat.stride(0)
+    ld = flat.stride(0)
+    if (flat.stride(1) != 1 and cols != 1) or (ld < cols and flat.shape[0] > 1):
+        flat, ld = flat.contiguous(), cols
+    return flat, flat.shape[0], max(ld, cols)
+
+
+def _mapped(t, ld):
+    """Whether the tensor maps read these rows as they lie (others are copied by the library)."""
+    return ld % 8 == 0 and t.data_ptr() % 16 == 0
 
 
 def _check(x, weight, act):
@@ -87,14 +76,18 @@ def _forward(x, weight, bias, act, residual, want_pre):
     if residual is not None:
         _same(residual, x, shape, "residual")
         res, _, ldr = _matrix(residual, n)
-    flat, rows, ldx = _operand(x, k)
-    w, _, ldw = _operand(weight, k)
+    flat, rows, ldx = _matrix(x, k)
+    w, _, ldw = _matrix(weight, k)
     y = torch.empty(shape, dtype=x.dtype, device=device)
     if want_pre:
         pre = torch.empty(shape, dtype=x.dtype, device=device)
+    need, ws = 0, None
+    if not (_mapped(flat, ldx) and _mapped(w, ldw)):
+        need = _lib.load().vdn_linear_workspace_size(flat.data_ptr(), ldx, w.data_ptr(), ldw, rows, n, k)
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
     _lib.call_on(device, "vdn_linear_act", flat.data_ptr(), ldx, w.data_ptr(), ldw, _lib.address(bias),
                  _lib.address(res), ldr, _lib.dtype_code(x.dtype), ACTIVATIONS[act], rows, n, k, y.data_ptr(), n,
-                 _lib.address(pre), n, _status(device).data_ptr())
+                 _lib.address(pre), n, _lib.address(ws), need, _status(device).data_ptr())
     return y, pre
 
 
@@ -120,8 +113,8 @@ def linear_act(x, weight, bias=None, *, act="none", residual=None, return_pre=Fa
     [..., n], all bf16 or all fp16; act is one of ACTIVATIONS.  With return_pre also
     x @ weight.T + bias, rounded (what linear_act_backward takes for an activation).
 
-    Row-strided operands are read in place where their rows are 16-byte aligned, others
-    (odd k, transposed) are copied into padded rows first."""
+    Row-strided operands are read in place where their rows are 16-byte aligned; the
+    library copies others (odd k, offset views) into padded rows first."""
     if torch.is_grad_enabled() and _lib.records(x, weight, bias, residual):
         if return_pre:
             raise ValueError("return_pre is for the explicit backward, not where gradients are recorded")
@@ -140,35 +133,22 @@ def _backward(grad_y, x, weight, pre, act, want_x, want_w, want_b):
         if pre is None:
             raise ValueError("pre (linear_act's return_pre) is needed for the activation's gradient")
         _same(pre, x, shape, "pre")
-    dev, code, word = x.device, _lib.dtype_code(x.dtype), _status(x.device).data_ptr()
-    dz, rows, ldz = _matrix(grad_y, n)
-    db = ws = z = None
-    need = ldp = 0
-    if want_b:
-        db = torch.empty(n, dtype=x.dtype, device=dev)
-        need = _lib.load().vdn_linear_dz_workspace_size(rows, n)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    dy, ldy = dz, ldz
+    dev, z, ldp = x.device, None, 0
+    dy, rows, ldy = _matrix(grad_y, n)
     if act != "none":
         z, _, ldp = _matrix(pre, n)
-        ldz = _pad8(n)
-        dz = torch.empty(rows, ldz, dtype=x.dtype, device=dev)[:, :n]
-    if want_b or act != "none":
-        _lib.call_on(dev, "vdn_linear_dz", dy.data_ptr(), ldy, _lib.address(z), ldp, code, ACTIVATIONS[act], rows, n,
-                     dz.data_ptr(), ldz, _lib.address(db), _lib.address(ws), need)
-    dx = dw = None
-    if want_x or want_w:
-        dz, _, ldz = _operand(dz, n)
-    if want_x:
-        w, _, ldw = _operand(weight, k)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        _lib.call_on(dev, "vdn_linear_dx", dz.data_ptr(), ldz, w.data_ptr(), ldw, code, rows, n, k, dx.data_ptr(), k,
-                     word)
-    if want_w:
-        flat, _, ldx = _operand(x, k)
-        dw = torch.empty(n, k, dtype=x.dtype, device=dev)
-        _lib.call_on(dev, "vdn_linear_dw", dz.data_ptr(), ldz, flat.data_ptr(), ldx, code, rows, n, k, dw.data_ptr(),
-                     k, word)
+    flat, _, ldx = _matrix(x, k)
+    w, _, ldw = _matrix(weight, k)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_x else None
+    dw = torch.empty(n, k, dtype=x.dtype, device=dev) if want_w else None
+    db = torch.empty(n, dtype=x.dtype, device=dev) if want_b else None
+    code = ACTIVATIONS[act]
+    need = _lib.load().vdn_linear_backward_workspace_size(dy.data_ptr(), ldy, flat.data_ptr(), ldx, w.data_ptr(), ldw,
+                                                          code, rows, n, k)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _lib.call_on(dev, "vdn_linear_act_backward", dy.data_ptr(), ldy, _lib.address(z), ldp, flat.data_ptr(), ldx,
+                 w.data_ptr(), ldw, _lib.dtype_code(x.dtype), code, rows, n, k, _lib.address(dx), k, _lib.address(dw), k,
+                 _lib.address(db), ws.data_ptr(), need, _status(dev).data_ptr())
     return dx, dw, db
 
 
