@@ -659,8 +659,8 @@ static void configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, int64_
 // 305 us with clusters of 8, which need 640 places where there are 592, and 282 us with 5),
 // and every CTA starts up anew.  Measured over clusters of one to eight, CTAs of four and
 // eight warps and nine shapes, a round takes about as long as 1 + (the warps on the fullest SM)
-// / 4, and starting up as two rounds; choosing by that was within a tenth of the best of
-// them.  The ring kernel's places decide for both kernels, so that the order of the sums does
+// / 4 (shared decays, which cost one evaluation per token instead of one per element: 2 + ..),
+// and starting up as two rounds; choosing by that was within a tenth of the best of them.  The ring kernel's places decide for both kernels, so that the order of the sums does
 // not hang on alignment.
 template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED>
 static int choose_shape(int64_t mean, int64_t longest, int64_t seqs, int64_t tiles, int& warps, int& cluster) {
@@ -686,7 +686,7 @@ static int choose_shape(int64_t mean, int64_t longest, int64_t seqs, int64_t til
         fit = n > 0 ? n : 1;
       }
       const int64_t waves = (ids + fit - 1) / fit, tail = ids - (waves - 1) * fit;
-      auto load = [&](int64_t clusters) { return 4 + w * ((clusters * c + 147) / 148); };
+      auto load = [&](int64_t clusters) { return (SHARED ? 8 : 4) + w * ((clusters * c + 147) / 148); };
       // the longest sequences' tiles go on alone
       const int64_t t = ((runs + c - 1) / c + 2) * ((waves - 1) * load(fit) + load(tail)) +
                         ((most_runs + c - 1) / c - (runs + c - 1) / c) * load(tiles);
