@@ -159,6 +159,21 @@ def test_same_bits_streams_and_graphs(cuda):
     assert all(torch.equal(p, q) and torch.equal(p, r) for p, q, r in zip(want, *outs))
 
 
+def test_offsets_past_32_bits(cuda):
+    from vdn_b200.layer_norm import layer_norm, layer_norm_backward
+    rows, width = 430000, 5120
+    x = torch.zeros(rows, width, dtype=torch.bfloat16, device=cuda)
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    x[-40:] = torch.randn(40, width, generator=gen, device=cuda).bfloat16()
+    w = torch.rand(width, generator=gen, device=cuda)
+    y, mean, rstd = layer_norm(x, w, w, return_stats=True)
+    assert torch.equal(y[-40:], layer_norm(x[-40:], w, w)) and torch.equal(y[:2], w.bfloat16().expand(2, width))
+    dx, dw, db = layer_norm_backward(x, x, w, mean, rstd)
+    ex, ew, eb = layer_norm_backward(x[-40:], x[-40:], w, mean[-40:], rstd[-40:])
+    assert torch.equal(dx[-40:], ex) and not bool(dx[:-40].any())
+    assert bool(((dw - ew).abs() <= 64 * U * (ew.abs() + 40)).all()) and bool(((db - eb).abs() <= 64 * U * 200).all())
+
+
 def test_gradients_against_differences(cuda):
     from vdn_b200.layer_norm import layer_norm
     gen = torch.Generator().manual_seed(1)

@@ -154,6 +154,27 @@ def test_strided_operands_and_shapes(cuda):
     assert torch.equal(linear_act(x, w, b, act="silu", residual=flat), want)
 
 
+def test_offsets_past_32_bits(cuda):
+    from vdn_b200.linear_act import linear_act, linear_act_backward
+    rows, n, k = 430000, 5120, 64
+    x, w, b, _, _ = (t.to(cuda) for t in _inputs(6, 64, n, k, torch.bfloat16))
+    big = torch.zeros(rows, k, dtype=torch.bfloat16, device=cuda)
+    big[-64:] = x
+    y, pre = linear_act(big, w, b, act="silu", return_pre=True)
+    few, few_pre = linear_act(x, w, b, act="silu", return_pre=True)
+    # two kernels, two orders of the sums: a rounding step of the result apart at most
+    assert bool(((y[-64:].float() - few.float()).abs() <= 2.0 ** -7 * few.float().abs() + 1e-4).all())
+    assert bool(((pre[-64:].float() - few_pre.float()).abs() <= 2.0 ** -7 * few_pre.float().abs() + 1e-4).all())
+    del y
+    dy = torch.zeros(rows, n, dtype=torch.bfloat16, device=cuda)
+    dy[-64:] = few
+    dx, dw, db = linear_act_backward(dy, big, w, pre, act="silu")
+    ex, ew, eb = linear_act_backward(few, x, w, few_pre, act="silu")
+    for p, q in ((dx[-64:], ex), (dw, ew), (db, eb)):
+        assert float((p.float() - q.float()).norm()) <= 2.0 ** -6 * float(q.float().norm())
+    assert not bool(dx[:-64].any())
+
+
 def test_large_values(cuda):
     """Saturated activations: no NaN from overflowing exponentials or cubes."""
     from vdn_b200.linear_act import linear_act, linear_act_backward

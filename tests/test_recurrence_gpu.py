@@ -218,6 +218,47 @@ def test_packed_out_keeps_rows_behind_the_last(cuda):
     assert bool((out[44:] == 3).all()) and not bool((out[:44] == 3).all())
 
 
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_rows_outside_the_sequences_do_not_matter(cuda, shared, reverse):
+    """NaN and infinities in front of the first sequence and behind the last."""
+    from vdn_b200.recurrence import gated_scan, gated_scan_backward
+    gen, x, g = _case(21, (500,), 2, 64, torch.bfloat16, torch.bfloat16, shared)
+    cu = torch.tensor([70, 75, 300, 431], dtype=torch.int32, device=cuda)
+    x, g = x.to(cuda), g.to(cuda)
+
+    def both():
+        y, last = gated_scan(x, g, cu_seqlens=cu, reverse=reverse)
+        return (y[70:431].clone(), last, *[t[70:431].clone() if t.dim() == x.dim() or t.shape == g.shape else t
+                                           for t in gated_scan_backward(x, g, y, cu_seqlens=cu, reverse=reverse)])
+    want = both()
+    for t in (x, g):
+        t[:70], t[431:] = float("nan"), float("inf")
+    got = both()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(bool(torch.isfinite(t).all()) for t in got)
+
+
+def test_offsets_past_32_bits(cuda):
+    """2.2e9 elements: the last rows equal a scan of their own from the state before them."""
+    from vdn_b200.recurrence import gated_scan, gated_scan_backward
+    n, c, tail = 430000, 5120, 64
+    x = torch.zeros(1, n, c, dtype=torch.bfloat16, device=cuda)
+    g = torch.full((1, n, c), -0.25, dtype=torch.bfloat16, device=cuda)
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    x[:, -tail:] = torch.randn(1, tail, c, generator=gen, device=cuda).bfloat16()
+    y, last = gated_scan(x, g)
+    want, wlast = gated_scan(x[:, -tail:].contiguous(), g[:, -tail:].contiguous())
+    assert not bool(y[:, :-tail].any())
+    err = 2.0 ** -8 * want.float().abs() + 1e-5
+    assert bool(((y[:, -tail:].float() - want.float()).abs() <= err).all())
+    assert float((last - wlast).abs().max()) < 1e-4
+    del x
+    dx, dg, _ = gated_scan_backward(y, g, y)
+    wx, wg, _ = gated_scan_backward(want, g[:, -tail:].contiguous(), want)
+    for a, b in ((dx, wx), (dg, wg)):
+        assert bool(((a[:, -tail:].float() - b.float()).abs() <= 2.0 ** -6 * b.float().abs() + 1e-3).all())
+
+
 def test_steps_continue_a_scan(cuda):
     """Token by token with the state in place equals one call over all tokens."""
     from vdn_b200.recurrence import gated_scan

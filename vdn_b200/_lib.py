@@ -155,7 +155,8 @@ def address(t: torch.Tensor | None):
 def refuse_captured_autograd(name: str) -> None:
     """A recorded graph must not span a stream capture: the engine runs the gradient
     accumulators of leaves that an eager graph still holds on that graph's stream, which is
-    not being captured.  So the differentiable ops refuse to record while capturing."""
+    not being captured.  So the differentiable ops neither record nor run their recorded
+    backward while the stream is captured."""
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"{name} does not record gradients during stream capture; capture the explicit "
                            f"forward and {name}_backward calls instead")

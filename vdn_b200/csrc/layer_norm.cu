@@ -757,12 +757,14 @@ static int forward(const Fwd& p, cudaStream_t stream) {
       if (n <= 12 * 512) return launch_row<T, TW, V, 12, 1, 0, 512, 1>(p, (n + 383) / 384 * 32, stream);
     }
   } else if (vec == 2) {
-    if (n <= 8 * 32) return launch_row<T, TW, 2, 8, 1, 32, 256, 4>(p, 256, stream);
-    if (n <= 24 * 32) return launch_row<T, TW, 2, 24, 1, 32, 256, 3>(p, 256, stream);
+    if (n <= 8 * 32) return launch_row<T, TW, 2, 8, 4, 32, 128, 4>(p, 128, stream);
+    if (n <= 16 * 32) return launch_row<T, TW, 2, 16, 2, 32, 128, 4>(p, 128, stream);
+    if (n <= 8 * 512) return launch_row<T, TW, 2, 8, 2, 0, 512, 2>(p, (n + 255) / 256 * 32, stream);
     if (n <= 16 * 1024) return launch_row<T, TW, 2, 16, 1, 0, 1024, 1>(p, (n + 511) / 512 * 32, stream);
   } else {
-    if (n <= 8 * 32) return launch_row<T, TW, 1, 8, 1, 32, 256, 4>(p, 256, stream);
-    if (n <= 24 * 32) return launch_row<T, TW, 1, 24, 1, 32, 256, 3>(p, 256, stream);
+    if (n <= 8 * 32) return launch_row<T, TW, 1, 8, 4, 32, 128, 4>(p, 128, stream);
+    if (n <= 16 * 32) return launch_row<T, TW, 1, 16, 2, 32, 128, 4>(p, 128, stream);
+    if (n <= 8 * 1024) return launch_row<T, TW, 1, 8, 2, 0, 1024, 1>(p, (n + 255) / 256 * 32, stream);
     if (n <= 16 * 1024) return launch_row<T, TW, 1, 16, 1, 0, 1024, 1>(p, (n + 511) / 512 * 32, stream);
   }
   forward_wide_kernel<T, TW><<<(unsigned)p.rows, 1024, 0, stream>>>(p);
@@ -771,10 +773,16 @@ static int forward(const Fwd& p, cudaStream_t stream) {
 }
 
 // CTAs of the backward, one line of partial sums each.  A CTA per row has about width / 16
-// threads, so narrower rows take more CTAs to fill 148 SMs.  The count depends on the
-// shape alone, so results do not vary.
-static int64_t line_count(int64_t rows, int64_t width) {
-  const int64_t lines = 2 * kSMs * (width >= 5120 ? 1 : width <= 512 ? 10 : 5120 / width);
+// threads, so narrower rows take more CTAs to fill 148 SMs (the 16-bit ring kernel: a warp
+// per 1280 columns, eight warps an SM).  The count depends on the shape and type alone, so
+// results do not vary.
+static int64_t plain_lines(int64_t width) { return 2 * kSMs * (width >= 5120 ? 1 : width <= 512 ? 10 : 5120 / width); }
+static int64_t ring_lines(int64_t width) {
+  const int64_t warps = (width + 1279) / 1280;
+  return kSMs * (warps >= 4 ? 2 : warps == 3 ? 3 : 8 / warps);
+}
+static int64_t line_count(int64_t rows, int64_t width) {   // the most that any kernel takes
+  const int64_t a = plain_lines(width), b = ring_lines(width), lines = a > b ? a : b;
   return rows < lines ? rows : lines;
 }
 constexpr int kGroupLines = 4 * kSMs;        // where a lane group takes a row: CTAs of several rows
@@ -791,9 +799,12 @@ static int launch_backward(const Bwd& p, int block, int lines, cudaStream_t stre
 constexpr int kSmemPerSM = 227 * 1024;
 template <typename T, typename TW, int VEC, int NV, int ROWS, int MAXT, int PER_SM, bool HELD>
 static int launch_ring(const Bwd& p, int block, int lines, cudaStream_t stream, bool& done) {
-  const int share = PER_SM * (MAXT / block < 1 ? 1 : MAXT / block);   // CTAs an SM, by their threads
-  const int64_t stage = 2ll * ROWS * p.width * sizeof(T), room = kSmemPerSM / (share < 12 ? share : 12) - 2048;
-  const int stages = (int)(room / stage < kMaxStages ? room / stage : kMaxStages);
+  const int64_t stage = 2ll * ROWS * p.width * sizeof(T);
+  int stages = 0;                                    // as many CTAs an SM as its threads allow, or fewer for two stages
+  for (int share = PER_SM * (MAXT / block < 1 ? 1 : MAXT / block); share >= 1 && stages < 2; --share) {
+    const int64_t n = (kSmemPerSM / share - 2048) / stage;
+    stages = (int)(n < kMaxStages ? n : kMaxStages);
+  }
   if (stages < 2) return VDN_OK;
   auto* kernel = backward_ring_kernel<T, TW, VEC, NV, ROWS, MAXT, PER_SM, HELD>;
   static bool set[64] = {};
@@ -801,7 +812,7 @@ static int launch_ring(const Bwd& p, int block, int lines, cudaStream_t stream, 
   VDN_CUDA_TRY(cudaGetDevice(&dev));
   VDN_CHECK_ARG(dev >= 0 && dev < 64, "device index out of range");
   if (!set[dev]) {
-    VDN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemPerSM - 4096));
+    VDN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemPerSM - 2048));
     set[dev] = true;
   }
   kernel<<<lines, block, stages * stage, stream>>>(p, stages);
@@ -811,27 +822,25 @@ static int launch_ring(const Bwd& p, int block, int lines, cudaStream_t stream, 
 }
 
 template <typename T, typename TW>
-static int backward(const Bwd& p, int lines, void* dw, void* db, cudaStream_t stream) {
+static int backward(const Bwd& p, void* dw, void* db, cudaStream_t stream) {
   constexpr int V = 16 / sizeof(T), M = sizeof(T) / 2;   // M: fp32 holds half the values per vector
   const int vec = vector_of<T>(p.width, {p.x_ld, p.dy_ld, p.dx_ld}, {p.x, p.dy, p.dx}, {p.w}, sizeof(TW));
-  const int n = p.width / vec, few = lines < kGroupLines ? lines : kGroupLines;
-  int rc = -1;
+  auto few_of = [&](int64_t most) { return (int)(p.rows < most ? p.rows : most); };
+  const int n = p.width / vec, few = few_of(kGroupLines);
+  int lines = few_of(plain_lines(p.width)), rc = -1;
   if (vec == V) {
+    bool done = false;
     if (n <= 8) rc = launch_backward<T, TW, V, 1, 8, 128, 4, true>(p, 128, lines = few, stream);
     else if (n <= 16) rc = launch_backward<T, TW, V, 1, 16, 128, 4, true>(p, 128, lines = few, stream);
     else if (n <= 32) rc = launch_backward<T, TW, V, 1, 32, 128, 4, true>(p, 128, lines = few, stream);
     else if (n <= 64) rc = launch_backward<T, TW, V, 2, 32, 128, 4, true>(p, 128, lines = few, stream);
-    else if (p.x_ld * sizeof(T) % 16 == 0 && p.dy_ld * sizeof(T) % 16 == 0) {   // (given by vec, said once more)
-      bool done = false;
-      int r = VDN_OK;
-      if (n <= 2 * M * 320) r = launch_ring<T, TW, V, 2 * M, 2 / M, 320, 2, true>(p, (n + 64 * M - 1) / (64 * M) * 32, lines, stream, done);
-      else if (n <= 4 * M * 512) r = launch_ring<T, TW, V, 4 * M, 1, 512, 1, false>(p, (n + 128 * M - 1) / (128 * M) * 32, lines, stream, done);
-      if (r != VDN_OK) return r;
-      if (done) rc = VDN_OK;
-    }
-    if (rc == VDN_OK) {
-    } else if (n <= 2 * M * 320) rc = launch_backward<T, TW, V, 2 * M, 0, 320, 2, sizeof(T) == 2>(p, (n + 64 * M - 1) / (64 * M) * 32, lines, stream);
-    else if (n <= 4 * M * 512) rc = launch_backward<T, TW, V, 4 * M, 0, 512, 1, false>(p, (n + 128 * M - 1) / (128 * M) * 32, lines, stream);
+    // 16 bits: few fat threads (40 columns, up to 255 registers) cost the fewest instructions a
+    // value (5120 columns: 183 us against 227 for 16 columns a thread); 32 bits: bound by HBM
+    else if (M == 1 && n <= 640) rc = launch_ring<T, TW, V, 5, 2, 128, 2, true>(p, (n + 159) / 160 * 32, lines = few_of(ring_lines(p.width)), stream, done);
+    else if (M == 2 && n <= 4 * 320) rc = launch_ring<T, TW, V, 4, 1, 320, 2, true>(p, (n + 127) / 128 * 32, lines, stream, done);
+    else if (n <= 4 * M * 512) rc = launch_ring<T, TW, V, 4 * M, 1, 512, 1, false>(p, (n + 128 * M - 1) / (128 * M) * 32, lines, stream, done);
+    if (n > 64 && n <= 4 * M * 512 && rc == VDN_OK && !done)   // rows too long for two stages
+      rc = launch_backward<T, TW, V, 4 * M, 0, 512, 1, false>(p, (n + 128 * M - 1) / (128 * M) * 32, lines, stream);
   } else if (vec == 2) {
     if (n <= 128) rc = launch_backward<T, TW, 2, 4, 32, 128, 4, true>(p, 128, lines = few, stream);
     else if (n <= 8 * 512) rc = launch_backward<T, TW, 2, 8, 0, 512, 1, true>(p, (n + 255) / 256 * 32, lines, stream);
@@ -904,8 +913,7 @@ extern "C" int vdn_layer_norm_backward(const void* dy, int dtype, int64_t rows, 
   VDN_CHECK_ARG(rows == 1 || (dy_stride >= 0 && x_stride >= 0 && dx_stride >= width), "bad row stride");
   VDN_CHECK_ARG(workspace_bytes >= vdn_layer_norm_backward_workspace_size(rows, width),
                 "workspace smaller than vdn_layer_norm_backward_workspace_size");
-  const int lines = (int)line_count(rows, width);
   const Bwd p = {dy, x, weight, mean, rstd, dx, static_cast<float*>(workspace), rows, dy_stride, x_stride, dx_stride,
                  (int)width, status};
-  VDN_LN_DISPATCH(backward, p, lines, d_weight, d_bias, stream)
+  VDN_LN_DISPATCH(backward, p, d_weight, d_bias, stream)
 }

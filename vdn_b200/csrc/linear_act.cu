@@ -60,6 +60,36 @@ __device__ __forceinline__ float act_slope(float z) {
   return (v >= 0.f ? r : e * r) + c * dv * (e * r * r);
 }
 
+// Two slopes at a time on packed pairs (gelu's tanh form and silu): the same formula with one
+// reciprocal for both, r0 = q (1 + e1), r1 = q (1 + e0), q = 1 / ((1 + e0) (1 + e1)).
+template <int ACT>
+__device__ __forceinline__ f2 act_slope2(f2 z) {
+  auto c2 = [](float v) { return f2_pack(v, v); };
+  float z0, z1;
+  f2_unpack(z, z0, z1);
+  if constexpr (ACT == NONE || ACT == ERF) return f2_pack(act_slope<ACT>(z0), act_slope<ACT>(z1));
+  asm("max.NaN.f32 %0, %0, 0fC1F00000;\n\tmin.NaN.f32 %0, %0, 0f41F00000;" : "+f"(z0));
+  asm("max.NaN.f32 %0, %0, 0fC1F00000;\n\tmin.NaN.f32 %0, %0, 0f41F00000;" : "+f"(z1));
+  const f2 c = f2_pack(z0, z1);
+  f2 v = c, cdv = c;                         // the sigmoid's argument, and c dv/dc
+  if constexpr (ACT == TANH) {
+    const float k = 1.5957691216057308f;
+    const f2 s = f2_mul(c, c);
+    v = f2_mul(c, f2_fma(s, c2(0.044715f * k), c2(k)));
+    cdv = f2_mul(c, f2_fma(s, c2(0.134145f * k), c2(k)));
+  }
+  float v0, v1, a, b, q0, q1, p0, p1;
+  f2_unpack(v, v0, v1);
+  f2_unpack(f2_mul(f2_pack(fabsf(v0), fabsf(v1)), c2(-1.4426950408889634f)), a, b);
+  const f2 e = f2_pack(ex2_approx(a), ex2_approx(b));
+  f2_unpack(f2_add(e, c2(1.0f)), a, b);
+  const float q = rcp_approx(a * b);
+  const f2 r = f2_mul(f2_pack(b, a), c2(q)), er = f2_mul(e, r);
+  f2_unpack(r, q0, q1);
+  f2_unpack(er, p0, p1);
+  return f2_fma(cdv, f2_mul(er, r), f2_pack(v0 >= 0.f ? q0 : p0, v1 >= 0.f ? q1 : p1));
+}
+
 // ------------------------------------------------------------------ shared pieces
 __device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                              uint32_t accumulate) {
@@ -636,9 +666,11 @@ __global__ void __launch_bounds__(256) dz_kernel(const T* dy, int64_t ldy, const
   const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 * VEC + lane * VEC;
   const int64_t r0 = (int64_t)blockIdx.y * chunk, r1 = min(r0 + chunk, rows);
-  float acc[VEC];
+  using V = typename Lanes<VEC>::V;
+  constexpr int NP = Lanes<VEC>::N;
+  V total[NP];
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+  for (int i = 0; i < NP; ++i) total[i] = vset(V{}, 0.f);
   if (c < cols) {
     constexpr int U = 4;                     // rows in flight
     for (int64_t r = r0 + g; r < r1; r += 8 * U) {
@@ -651,20 +683,25 @@ __global__ void __launch_bounds__(256) dz_kernel(const T* dy, int64_t ldy, const
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        float d[VEC];
-        unpack<T, VEC>(a[u], d);
+        V d[NP];
+        unpack_lanes<T, VEC>(a[u], d);
         if constexpr (ACT != NONE) {
-          float z[VEC];
-          unpack<T, VEC>(b[u], z);
+          V z[NP];
+          unpack_lanes<T, VEC>(b[u], z);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) d[i] *= act_slope<ACT>(z[i]);
-          if (r + 8 * u < r1) *reinterpret_cast<R*>(dz + (r + 8 * u) * ldz + c) = pack<T, VEC>(d);
+          for (int i = 0; i < NP; ++i) {
+            if constexpr (VEC == 1) d[i] = vmul(d[i], act_slope<ACT>(z[i]));
+            else d[i] = vmul(d[i], act_slope2<ACT>(z[i]));
+          }
+          if (r + 8 * u < r1) *reinterpret_cast<R*>(dz + (r + 8 * u) * ldz + c) = pack_lanes<T, VEC>(d);
         }
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] += d[i];
+        for (int i = 0; i < NP; ++i) total[i] = vadd(total[i], d[i]);
       }
     }
   }
+  float acc[VEC];
+  from_lanes(total, acc);
   if (!part) return;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) sums[g][lane * VEC + i] = acc[i];
@@ -876,8 +913,12 @@ static int forward(const void* x, int64_t ldx, const void* w, int64_t ldw, int64
   return product<T, false, false, ACT>({x, ldx, false}, {w, ldw, false}, k, p, s);
 }
 
-constexpr int64_t kChunks = 64;              // row chunks of the bias gradient, at most
-static int64_t chunk_rows(int64_t rows) { return (((rows + kChunks - 1) / kChunks) + 31) / 32 * 32; }
+// Row chunks of the bias gradient, at most: 64, or as many as give narrow outputs eight CTAs an SM.
+static int64_t chunk_count(int64_t n) {
+  const int64_t c = 8 * 148 / ((n + 255) / 256);
+  return c > 64 ? c : 64;
+}
+static int64_t chunk_rows(int64_t rows, int64_t n) { return (((rows + chunk_count(n) - 1) / chunk_count(n)) + 31) / 32 * 32; }
 
 template <typename T, int ACT>
 static int dz_run(const void* dy, int64_t ldy, const void* pre, int64_t ldp, void* dz, int64_t ldz, int64_t rows,
@@ -885,7 +926,7 @@ static int dz_run(const void* dy, int64_t ldy, const void* pre, int64_t ldp, voi
   constexpr int V = 8;
   auto ok = [&](const void* q, int64_t ld) { return !q || (aligned16(q) && ld % V == 0); };
   const bool vec = n % V == 0 && ok(dy, ldy) && ok(pre, ldp) && ok(dz, ldz);
-  const int64_t chunk = chunk_rows(rows), chunks = (rows + chunk - 1) / chunk;
+  const int64_t chunk = chunk_rows(rows, n), chunks = (rows + chunk - 1) / chunk;
   float* to = db ? part : nullptr;
   if (ACT != NONE || db) {
     if (vec)
@@ -959,7 +1000,7 @@ namespace lact {
 static size_t dz_bytes(const void* dy, int64_t ldy, int act, int64_t rows, int64_t n) {
   return act != NONE ? ((size_t)rows * pad8(n) * 2 + 255) / 256 * 256 : padded_bytes(dy, ldy, rows, n);
 }
-static size_t part_bytes(int64_t n) { return (sizeof(float) * kChunks * (size_t)n + 255) / 256 * 256; }
+static size_t part_bytes(int64_t n) { return (sizeof(float) * (size_t)chunk_count(n) * (size_t)n + 255) / 256 * 256; }
 
 template <typename T>
 static int backward(const void* dy, int64_t ldy, const void* pre, int64_t ldp, const void* x, int64_t ldx,

@@ -17,7 +17,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .mxfp8_linear import _status
+from .mxfp8_linear import status_address
 
 __all__ = ["layer_norm", "layer_norm_backward"]
 
@@ -91,6 +91,7 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_y):
+        _lib.refuse_captured_autograd("layer_norm")
         x, weight, bias, mean, rstd = ctx.saved_tensors
         dx, dw, db = _backward(grad_y, x, weight, mean, rstd, ctx.needs_input_grad[1], ctx.needs_input_grad[2],
                                None if bias is None else bias.dtype)
@@ -129,7 +130,7 @@ def _backward(grad_y, x, weight, mean, rstd, want_w, want_b, bias_dtype=None):
     _lib.call_on(x.device, "vdn_layer_norm_backward", dy.data_ptr(), _lib.dtype_code(x.dtype), rows, width, dy_ld,
                  flat.data_ptr(), x_ld, _lib.address(w), _lib.dtype_code(kind), mean.data_ptr(), rstd.data_ptr(),
                  dx.data_ptr(), width, _lib.address(dw), _lib.address(db), ws.data_ptr(), need,
-                 _status(x.device).data_ptr())
+                 status_address(x.device))
     return dx, dw, db
 
 

@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .mxfp8_linear import _status
+from .mxfp8_linear import status_address
 
 __all__ = ["linear_act", "linear_act_backward", "ACTIVATIONS"]
 
@@ -87,7 +87,7 @@ def _forward(x, weight, bias, act, residual, want_pre):
         ws = torch.empty(need, dtype=torch.uint8, device=device)
     _lib.call_on(device, "vdn_linear_act", flat.data_ptr(), ldx, w.data_ptr(), ldw, _lib.address(bias),
                  _lib.address(res), ldr, _lib.dtype_code(x.dtype), ACTIVATIONS[act], rows, n, k, y.data_ptr(), n,
-                 _lib.address(pre), n, _lib.address(ws), need, _status(device).data_ptr())
+                 _lib.address(pre), n, _lib.address(ws), need, status_address(device))
     return y, pre
 
 
@@ -102,6 +102,7 @@ class _LinearAct(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_y):
+        _lib.refuse_captured_autograd("linear_act")
         x, weight, pre = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx, dw, db = _backward(grad_y, x, weight, pre, ctx.act, need[0], need[1], need[2])
@@ -148,7 +149,7 @@ def _backward(grad_y, x, weight, pre, act, want_x, want_w, want_b):
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     _lib.call_on(dev, "vdn_linear_act_backward", dy.data_ptr(), ldy, _lib.address(z), ldp, flat.data_ptr(), ldx,
                  w.data_ptr(), ldw, _lib.dtype_code(x.dtype), code, rows, n, k, _lib.address(dx), k, _lib.address(dw), k,
-                 _lib.address(db), ws.data_ptr(), need, _status(dev).data_ptr())
+                 _lib.address(db), ws.data_ptr(), need, status_address(dev))
     return dx, dw, db
 
 

@@ -61,6 +61,14 @@ def _status(device) -> torch.Tensor:
     return word
 
 
+def status_address(device):
+    """The address of the device's status word for ops that may be captured: None where the
+    word does not exist yet and a capture would put it into the graph's memory."""
+    if device.index not in _STATUS and torch.cuda.is_current_stream_capturing():
+        return None
+    return _status(device).data_ptr()
+
+
 def mxfp8_gemm(data, scales, weight_data, weight_scale, n, *, rows, bias=None, out=None):
     """y[:rows, :n] = bf16(dequant(data) dequant(weight)^T) (+ bias) on tcgen05."""
     m_pad, k_pad = data.shape

@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .mxfp8_linear import _status
+from .mxfp8_linear import status_address
 
 __all__ = ["gated_scan", "gated_scan_backward"]
 
@@ -113,7 +113,7 @@ def _forward(x, log_decay, state, cu_seqlens, reverse, out, out_state):
     _lib.call_on(device, "vdn_gated_scan", x.data_ptr(), _lib.dtype_code(x.dtype), x_batch, x_row,
                  log_decay.data_ptr(), _lib.dtype_code(log_decay.dtype), g_batch, g_row, shared, _lib.address(state),
                  _lib.address(cu_seqlens), seqs, rows, heads, d, reverse, y.data_ptr(), y_batch, y_row, out is None,
-                 out_state.data_ptr(), _status(device).data_ptr())
+                 out_state.data_ptr(), status_address(device))
     return y, out_state
 
 
@@ -129,6 +129,7 @@ class _GatedScan(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_y, grad_last):
+        _lib.refuse_captured_autograd("gated_scan")
         log_decay, y, state, cu_seqlens = ctx.saved_tensors
         if grad_y is None:
             grad_y = torch.zeros_like(y)
@@ -188,5 +189,5 @@ def gated_scan_backward(grad_y, log_decay, y, *, state=None, grad_state=None, cu
                  log_decay.data_ptr(), _lib.dtype_code(log_decay.dtype), g_batch, g_row, shared, y.data_ptr(), y_batch,
                  y_row, _lib.address(state), _lib.address(grad_state), _lib.address(cu_seqlens), seqs, rows, heads, d,
                  bool(reverse), dx.data_ptr(), dx_batch, dx_row, dg.data_ptr(), dg_batch, dg_row, True,
-                 ds.data_ptr(), _status(device).data_ptr())
+                 ds.data_ptr(), status_address(device))
     return dx, dg, ds
