@@ -152,12 +152,22 @@ def address(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
-def refuse_captured_autograd(name: str) -> None:
+def capturing(device: torch.device) -> bool:
+    """Whether `device`'s current stream is being captured."""
+    if device.type != "cuda":
+        return False
+    if device.index == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
+def refuse_captured_autograd(name: str, t: torch.Tensor) -> None:
     """A recorded graph must not span a stream capture: the engine runs the gradient
     accumulators of leaves that an eager graph still holds on that graph's stream, which is
     not being captured.  So the differentiable ops neither record nor run their recorded
     backward while the stream is captured."""
-    if torch.cuda.is_current_stream_capturing():
+    if capturing(t.device):
         raise RuntimeError(f"{name} does not record gradients during stream capture; capture the explicit "
                            f"forward and {name}_backward calls instead")
 

@@ -91,7 +91,7 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_y):
-        _lib.refuse_captured_autograd("layer_norm")
+        _lib.refuse_captured_autograd("layer_norm", ctx.saved_tensors[0])
         x, weight, bias, mean, rstd = ctx.saved_tensors
         dx, dw, db = _backward(grad_y, x, weight, mean, rstd, ctx.needs_input_grad[1], ctx.needs_input_grad[2],
                                None if bias is None else bias.dtype)
@@ -104,7 +104,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, return_stats=False):
     if torch.is_grad_enabled() and _lib.records(x, weight, bias):
         if return_stats:
             raise ValueError("return_stats is for the explicit backward, not where gradients are recorded")
-        _lib.refuse_captured_autograd("layer_norm")
+        _lib.refuse_captured_autograd("layer_norm", x)
         return _LayerNorm.apply(x, weight, bias, float(eps))
     y, mean, rstd = _forward(x, weight, bias, eps, return_stats)
     return (y, mean, rstd) if return_stats else y

@@ -102,7 +102,7 @@ class _LinearAct(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_y):
-        _lib.refuse_captured_autograd("linear_act")
+        _lib.refuse_captured_autograd("linear_act", ctx.saved_tensors[0])
         x, weight, pre = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx, dw, db = _backward(grad_y, x, weight, pre, ctx.act, need[0], need[1], need[2])
@@ -119,7 +119,7 @@ def linear_act(x, weight, bias=None, *, act="none", residual=None, return_pre=Fa
     if torch.is_grad_enabled() and _lib.records(x, weight, bias, residual):
         if return_pre:
             raise ValueError("return_pre is for the explicit backward, not where gradients are recorded")
-        _lib.refuse_captured_autograd("linear_act")
+        _lib.refuse_captured_autograd("linear_act", x)
         return _LinearAct.apply(x, weight, bias, act, residual)
     y, pre = _forward(x, weight, bias, act, residual, return_pre)
     return (y, pre) if return_pre else y

@@ -64,7 +64,7 @@ def _status(device) -> torch.Tensor:
 def status_address(device):
     """The address of the device's status word for ops that may be captured: None where the
     word does not exist yet and a capture would put it into the graph's memory."""
-    if device.index not in _STATUS and torch.cuda.is_current_stream_capturing():
+    if device.index not in _STATUS and _lib.capturing(device):
         return None
     return _status(device).data_ptr()
 

@@ -129,7 +129,7 @@ class _GatedScan(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_y, grad_last):
-        _lib.refuse_captured_autograd("gated_scan")
+        _lib.refuse_captured_autograd("gated_scan", ctx.saved_tensors[0])
         log_decay, y, state, cu_seqlens = ctx.saved_tensors
         if grad_y is None:
             grad_y = torch.zeros_like(y)
@@ -153,7 +153,7 @@ def gated_scan(x, log_decay, state=None, *, cu_seqlens=None, reverse=False, out=
     if torch.is_grad_enabled() and _lib.records(x, log_decay, state):
         if out is not None or out_state is not None:
             raise ValueError("out and out_state cannot be given where gradients are recorded")
-        _lib.refuse_captured_autograd("gated_scan")
+        _lib.refuse_captured_autograd("gated_scan", x)
         return _GatedScan.apply(x, log_decay, state, cu_seqlens, bool(reverse))
     return _forward(x, log_decay, state, cu_seqlens, bool(reverse), out, out_state)
 
