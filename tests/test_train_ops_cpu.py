@@ -116,23 +116,23 @@ def test_calls_run_on_the_tensors_device(monkeypatch):
 
     class Device:
         def __init__(self, d):
-            self.d = d.index
+            self.d = d
 
         def __enter__(self):
             self.before, current[0] = current[0], self.d
 
         def __exit__(self, *exc):
             current[0] = self.before
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(_lib, "_current_device", lambda: current[0])
     monkeypatch.setattr(torch.cuda, "device", Device)
     monkeypatch.setattr(_lib, "_raw_stream", lambda index: 1000 + index)
     monkeypatch.setitem(_lib._FUNCTIONS, "vdn_fake", lambda *a: seen.append((current[0], a)) or 0)
-    _lib.call_on(torch.device("cuda", 0), "vdn_fake", 5)
-    _lib.call_on(torch.device("cuda", 3), "vdn_fake", 6)
+    _lib.call_on(0, "vdn_fake", 5)
+    _lib.call_on(3, "vdn_fake", 6)
     assert seen == [(0, (5, 1000)), (3, (6, 1003))] and current == [0]
     monkeypatch.setitem(_lib._FUNCTIONS, "vdn_fake", lambda *a: _lib.VDN_ERR_VALUE)
     with pytest.raises(ValueError):
-        _lib.call_on(torch.device("cuda", 3), "vdn_fake")
+        _lib.call_on(3, "vdn_fake")
     assert current == [0]
 
 

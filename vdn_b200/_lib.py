@@ -122,22 +122,30 @@ def call(name: str, *args) -> int:
 _FUNCTIONS: dict[str, object] = {}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def call_on(device: torch.device, name: str, *args) -> None:
-    """The entry point `name` with `device` current and its current stream as last argument
+def call_on(index: int, name: str, *args) -> None:
+    """The entry point `name` with device `index` current and its current stream as last argument
     (pointers as plain addresses: the short path of the ops whose calls cost microseconds)."""
     fn = _FUNCTIONS.get(name)
     if fn is None:
         fn = _FUNCTIONS[name] = getattr(load(), name)
-    index = device.index
-    if index == torch.cuda.current_device():
+    if index == _current_device():
         rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             rc = fn(*args, _raw_stream(index))
     if rc != VDN_OK:
         raise_status(rc)
+
+
+def device_index(t: torch.Tensor, what: str) -> int:
+    """The index of t's device, which must be an sm_100 CUDA device."""
+    index = t.get_device()
+    if index < 0 or not _SUPPORTED.get(index):
+        require_device(t, what)
+    return index
 
 
 def records(*tensors) -> bool:
@@ -206,11 +214,11 @@ def require_device(t: torch.Tensor, what: str = "tensor") -> None:
         raise RuntimeError("vdn_b200 kernels require an sm_100 (B200) GPU; no fallback")
 
 
-_DTYPE_CODES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
+DTYPE_CODES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
 
 
 def dtype_code(dtype: torch.dtype) -> int:
     try:
-        return _DTYPE_CODES[dtype]
+        return DTYPE_CODES[dtype]
     except KeyError:
         raise TypeError(f"unsupported dtype {dtype}") from None

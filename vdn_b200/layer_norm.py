@@ -21,17 +21,13 @@ from .mxfp8_linear import status_address
 
 __all__ = ["layer_norm", "layer_norm_backward"]
 
-_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
-
-
 @functools.lru_cache(maxsize=1024)
 def _workspace_size(rows, width):
     return _lib.load().vdn_layer_norm_backward_workspace_size(rows, width)
 
 
-def _rows(t):
+def _rows(t, width):
     """(t as rows of unit column stride, a view where the layout allows it; rows; row stride)"""
-    width = t.shape[-1]
     if t.is_contiguous():
         return t, t.numel() // width, width
     flat = t.reshape(-1, width)
@@ -41,43 +37,50 @@ def _rows(t):
 
 
 def _check(x, weight, bias):
-    if not isinstance(x, torch.Tensor) or x.dtype not in _DTYPES:
+    """(device index, width, x's dtype code, the parameters' dtype code) of valid arguments."""
+    code = _lib.DTYPE_CODES.get(x.dtype) if isinstance(x, torch.Tensor) else None
+    if code is None:
         raise TypeError("x must be an fp32, bf16 or fp16 tensor")
-    if not x.is_cuda:
+    index = x.get_device()
+    if index < 0:
         raise ValueError("x must be a CUDA tensor")
-    if x.dim() < 1 or x.shape[-1] < 1:
+    index = _lib.device_index(x, "x")
+    width = x.shape[-1] if x.dim() else 0
+    if width < 1:
         raise ValueError("x must have a last dimension to normalise")
-    _lib.require_device(x, "x")
-    if weight is not None:
-        _check_parameter(x, weight, "weight")
-    if bias is not None:
-        _check_parameter(x, bias, "bias")
-        if weight is not None and weight.dtype != bias.dtype:
+    w_code = None
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is None:
+            continue
+        kind = _lib.DTYPE_CODES.get(t.dtype)
+        if kind != code and kind != _lib.DTYPE_F32:
+            raise TypeError(f"{name} must be {x.dtype} or fp32, got {t.dtype}")
+        if t.dim() != 1 or t.numel() != width or t.get_device() != index:
+            raise ValueError(f"{name} must be [{width}] on x's device")
+        if w_code is not None and kind != w_code:
             raise TypeError("weight and bias must share one dtype")
+        w_code = kind
+    return index, width, code, code if w_code is None else w_code
 
 
-def _check_parameter(x, t, name):
-    if t.dtype != x.dtype and t.dtype != torch.float32:
-        raise TypeError(f"{name} must be {x.dtype} or fp32, got {t.dtype}")
-    if t.dim() != 1 or t.shape[0] != x.shape[-1] or t.device != x.device:
-        raise ValueError(f"{name} must be [{x.shape[-1]}] on x's device")
+def _like(t):
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _forward(x, weight, bias, eps, stats):
-    _check(x, weight, bias)
-    flat, rows, ld = _rows(x)
-    width = x.shape[-1]
-    device, code = x.device, _lib.dtype_code(x.dtype)
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
-    mean = rstd = None
+    index, width, code, w_code = _check(x, weight, bias)
+    flat, rows, ld = _rows(x, width)
+    y = _like(x)
+    mean = rstd = w = b = None
     if stats:
-        mean, rstd = torch.empty(2, rows, dtype=torch.float32, device=device)
-    given = weight if weight is not None else bias
-    w = None if weight is None else weight.contiguous()
-    b = None if bias is None else bias.contiguous()
-    _lib.call_on(device, "vdn_layer_norm", flat.data_ptr(), code, rows, width, ld, _lib.address(w), _lib.address(b),
-                 code if given is None else _lib.dtype_code(given.dtype), eps, y.data_ptr(), width,
-                 _lib.address(mean), _lib.address(rstd))
+        mean, rstd = torch.empty(2, rows, dtype=torch.float32, device=x.device)
+    if weight is not None:
+        w = weight if weight.is_contiguous() else weight.contiguous()
+    if bias is not None:
+        b = bias if bias.is_contiguous() else bias.contiguous()
+    _lib.call_on(index, "vdn_layer_norm", flat.data_ptr(), code, rows, width, ld, w.data_ptr() if w is not None else None,
+                 b.data_ptr() if b is not None else None, w_code, eps, y.data_ptr(), width,
+                 mean.data_ptr() if stats else None, rstd.data_ptr() if stats else None)
     return y, mean, rstd
 
 
@@ -111,32 +114,36 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, return_stats=False):
 
 
 def _backward(grad_y, x, weight, mean, rstd, want_w, want_b, bias_dtype=None):
-    _check(x, weight, None)
-    if grad_y.shape != x.shape or grad_y.dtype != x.dtype or grad_y.device != x.device:
+    index, width, code, kind = _check(x, weight, None)
+    if grad_y.shape != x.shape or grad_y.dtype != x.dtype or grad_y.get_device() != index:
         raise ValueError("grad_y must match x in shape, dtype and device")
-    (flat, rows, x_ld), (dy, _, dy_ld) = _rows(x), _rows(grad_y)
-    width = x.shape[-1]
+    (flat, rows, x_ld), (dy, _, dy_ld) = _rows(x, width), _rows(grad_y, width)
     for t, name in ((mean, "mean"), (rstd, "rstd")):
-        if t.shape != (rows,) or t.dtype != torch.float32 or t.device != x.device:
+        if t.dtype != torch.float32 or t.dim() != 1 or t.numel() != rows or t.get_device() != index:
             raise ValueError(f"{name} must be fp32 [{rows}] on x's device")
-    kind = weight.dtype if weight is not None else bias_dtype or x.dtype
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dw = torch.empty(width, dtype=kind, device=x.device) if want_w else None
-    db = torch.empty(width, dtype=kind, device=x.device) if want_b else None
+    device, dtype = x.device, x.dtype if weight is None else weight.dtype
+    if weight is None and bias_dtype is not None:
+        dtype, kind = bias_dtype, _lib.dtype_code(bias_dtype)
+    dx = _like(x)
+    dw = torch.empty(width, dtype=dtype, device=device) if want_w else None
+    db = torch.empty(width, dtype=dtype, device=device) if want_b else None
     need = _workspace_size(rows, width)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
     w = None if weight is None else weight.contiguous()
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    _lib.call_on(x.device, "vdn_layer_norm_backward", dy.data_ptr(), _lib.dtype_code(x.dtype), rows, width, dy_ld,
-                 flat.data_ptr(), x_ld, _lib.address(w), _lib.dtype_code(kind), mean.data_ptr(), rstd.data_ptr(),
-                 dx.data_ptr(), width, _lib.address(dw), _lib.address(db), ws.data_ptr(), need,
-                 status_address(x.device))
+    _lib.call_on(index, "vdn_layer_norm_backward", dy.data_ptr(), code, rows, width, dy_ld, flat.data_ptr(), x_ld,
+                 None if w is None else w.data_ptr(), kind, mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), width,
+                 dw.data_ptr() if want_w else None, db.data_ptr() if want_b else None, ws.data_ptr(), need,
+                 status_address(device))
     return dx, dw, db
 
 
-@torch.no_grad()
 def layer_norm_backward(grad_y, x, weight, mean, rstd, *, bias=True):
     """(grad of x, of weight, of bias) from the forward's statistics; the weight's is None
     where there is no weight, the bias's unless `bias`.  Parameter gradients come in the
-    weight's dtype (x's without one), summed over the rows in fp32 in a fixed order."""
+    weight's dtype (x's without one), summed over the rows in fp32 in a fixed order.
+    Records nothing for autograd."""
+    if torch.is_grad_enabled():
+        with torch.no_grad():
+            return _backward(grad_y, x, weight, mean, rstd, weight is not None, bool(bias))
     return _backward(grad_y, x, weight, mean, rstd, weight is not None, bool(bias))

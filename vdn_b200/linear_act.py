@@ -35,17 +35,15 @@ def _matrix(t, cols):
     return flat, flat.shape[0], max(ld, cols)
 
 
-def _mapped(t, ld):
-    """Whether the tensor maps read these rows as they lie (others are copied by the library)."""
-    return ld % 8 == 0 and t.data_ptr() % 16 == 0
-
-
 def _check(x, weight, act):
+    """(device index, dtype code) of valid arguments."""
     if not isinstance(x, torch.Tensor) or not isinstance(weight, torch.Tensor):
         raise TypeError("x and weight must be tensors")
-    if (x.dtype != torch.bfloat16 and x.dtype != torch.float16) or weight.dtype != x.dtype:
+    dtype = x.dtype
+    if (dtype != torch.bfloat16 and dtype != torch.float16) or weight.dtype != dtype:
         raise TypeError(f"x and weight must both be bf16 or both fp16, got {x.dtype} and {weight.dtype}")
-    if not x.is_cuda or weight.device != x.device:
+    index = x.get_device()
+    if index < 0 or weight.get_device() != index:
         raise ValueError("x and weight must be CUDA tensors on one device")
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError("x must be [..., k] and weight [n, k]")
@@ -53,41 +51,42 @@ def _check(x, weight, act):
         raise ValueError("weight must not be empty")
     if act not in ACTIVATIONS:
         raise ValueError(f"act must be one of {tuple(ACTIVATIONS)}, got {act!r}")
-    _lib.require_device(x, "x")
+    return _lib.device_index(x, "x"), _lib.DTYPE_CODES[dtype]
 
 
-def _same(t, x, shape, name):
-    if t.dtype != x.dtype or t.device != x.device:
+def _same(t, x, index, shape, name):
+    if t.dtype != x.dtype or t.get_device() != index:
         raise TypeError(f"{name} must have x's dtype and device")
     if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
 
 
 def _forward(x, weight, bias, act, residual, want_pre):
-    _check(x, weight, act)
+    index, code = _check(x, weight, act)
     n, k = weight.shape
     shape = (*x.shape[:-1], n)
     device = x.device
-    res = pre = None
-    ldr = 0
+    res = pre = ws = None
+    ldr = need = 0
     if bias is not None:
-        _same(bias, x, (n,), "bias")
-        bias = bias.contiguous()
+        _same(bias, x, index, (n,), "bias")
+        bias = bias if bias.is_contiguous() else bias.contiguous()
     if residual is not None:
-        _same(residual, x, shape, "residual")
+        _same(residual, x, index, shape, "residual")
         res, _, ldr = _matrix(residual, n)
     flat, rows, ldx = _matrix(x, k)
     w, _, ldw = _matrix(weight, k)
     y = torch.empty(shape, dtype=x.dtype, device=device)
     if want_pre:
         pre = torch.empty(shape, dtype=x.dtype, device=device)
-    need, ws = 0, None
-    if not (_mapped(flat, ldx) and _mapped(w, ldw)):
-        need = _lib.load().vdn_linear_workspace_size(flat.data_ptr(), ldx, w.data_ptr(), ldw, rows, n, k)
+    px, pw = flat.data_ptr(), w.data_ptr()
+    if ldx % 8 or ldw % 8 or px % 16 or pw % 16:     # rows the tensor maps do not take: room for copies
+        need = _lib.load().vdn_linear_workspace_size(px, ldx, pw, ldw, rows, n, k)
         ws = torch.empty(need, dtype=torch.uint8, device=device)
-    _lib.call_on(device, "vdn_linear_act", flat.data_ptr(), ldx, w.data_ptr(), ldw, _lib.address(bias),
-                 _lib.address(res), ldr, _lib.dtype_code(x.dtype), ACTIVATIONS[act], rows, n, k, y.data_ptr(), n,
-                 _lib.address(pre), n, _lib.address(ws), need, status_address(device))
+    _lib.call_on(index, "vdn_linear_act", px, ldx, pw, ldw, None if bias is None else bias.data_ptr(),
+                 None if res is None else res.data_ptr(), ldr, code, ACTIVATIONS[act], rows, n, k, y.data_ptr(), n,
+                 None if pre is None else pre.data_ptr(), n, None if ws is None else ws.data_ptr(), need,
+                 status_address(device))
     return y, pre
 
 
@@ -126,36 +125,38 @@ def linear_act(x, weight, bias=None, *, act="none", residual=None, return_pre=Fa
 
 
 def _backward(grad_y, x, weight, pre, act, want_x, want_w, want_b):
-    _check(x, weight, act)
+    index, dtype = _check(x, weight, act)
     n, k = weight.shape
     shape = (*x.shape[:-1], n)
-    _same(grad_y, x, shape, "grad_y")
+    _same(grad_y, x, index, shape, "grad_y")
+    z, ldp = None, 0
     if act != "none":
         if pre is None:
             raise ValueError("pre (linear_act's return_pre) is needed for the activation's gradient")
-        _same(pre, x, shape, "pre")
-    dev, z, ldp = x.device, None, 0
-    dy, rows, ldy = _matrix(grad_y, n)
-    if act != "none":
+        _same(pre, x, index, shape, "pre")
         z, _, ldp = _matrix(pre, n)
+    dev, code = x.device, ACTIVATIONS[act]
+    dy, rows, ldy = _matrix(grad_y, n)
     flat, _, ldx = _matrix(x, k)
     w, _, ldw = _matrix(weight, k)
     dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_x else None
     dw = torch.empty(n, k, dtype=x.dtype, device=dev) if want_w else None
     db = torch.empty(n, dtype=x.dtype, device=dev) if want_b else None
-    code = ACTIVATIONS[act]
-    need = _lib.load().vdn_linear_backward_workspace_size(dy.data_ptr(), ldy, flat.data_ptr(), ldx, w.data_ptr(), ldw,
-                                                          code, rows, n, k)
+    pdy, px, pw = dy.data_ptr(), flat.data_ptr(), w.data_ptr()
+    need = _lib.load().vdn_linear_backward_workspace_size(pdy, ldy, px, ldx, pw, ldw, code, rows, n, k)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    _lib.call_on(dev, "vdn_linear_act_backward", dy.data_ptr(), ldy, _lib.address(z), ldp, flat.data_ptr(), ldx,
-                 w.data_ptr(), ldw, _lib.dtype_code(x.dtype), code, rows, n, k, _lib.address(dx), k, _lib.address(dw), k,
-                 _lib.address(db), ws.data_ptr(), need, status_address(dev))
+    _lib.call_on(index, "vdn_linear_act_backward", pdy, ldy, None if z is None else z.data_ptr(), ldp, px, ldx, pw, ldw,
+                 dtype, code, rows, n, k, dx.data_ptr() if want_x else None, k, dw.data_ptr() if want_w else None, k,
+                 db.data_ptr() if want_b else None, ws.data_ptr(), need, status_address(dev))
     return dx, dw, db
 
 
-@torch.no_grad()
 def linear_act_backward(grad_y, x, weight, pre=None, *, act="none", bias=True):
     """(grad of x, of weight, of bias or None) from the forward's inputs and `pre`.  The residual's
     gradient is grad_y.  The activation's gradient enters the two products rounded to the
-    operands' type; the bias gradient sums it unrounded, in fp32 and a fixed order."""
+    operands' type; the bias gradient sums it unrounded, in fp32 and a fixed order.  Records
+    nothing for autograd."""
+    if torch.is_grad_enabled():
+        with torch.no_grad():
+            return _backward(grad_y, x, weight, pre, act, True, True, bool(bias))
     return _backward(grad_y, x, weight, pre, act, True, True, bool(bias))

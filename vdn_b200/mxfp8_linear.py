@@ -64,9 +64,12 @@ def _status(device) -> torch.Tensor:
 def status_address(device):
     """The address of the device's status word for ops that may be captured: None where the
     word does not exist yet and a capture would put it into the graph's memory."""
-    if device.index not in _STATUS and _lib.capturing(device):
-        return None
-    return _status(device).data_ptr()
+    word = _STATUS.get(device.index)
+    if word is None:
+        if _lib.capturing(device):
+            return None
+        word = _status(device)
+    return word.data_ptr()
 
 
 def mxfp8_gemm(data, scales, weight_data, weight_scale, n, *, rows, bias=None, out=None):

@@ -20,20 +20,20 @@ from .mxfp8_linear import status_address
 
 __all__ = ["gated_scan", "gated_scan_backward"]
 
-_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
-
-
 def _layout(x, log_decay, state, cu_seqlens, what):
-    """(lead dims, sequences, rows, heads, head dim, shared decay) after the argument checks."""
+    """(device index, dtype codes, lead dims, sequences, rows, heads, head dim, shared decay,
+    state shape) after the argument checks."""
     if not isinstance(x, torch.Tensor) or not isinstance(log_decay, torch.Tensor):
         raise TypeError(f"{what} and log_decay must be tensors")
-    if x.dtype not in _DTYPES:
+    code, g_code = _lib.DTYPE_CODES.get(x.dtype), _lib.DTYPE_CODES.get(log_decay.dtype)
+    if code is None:
         raise TypeError(f"{what} must be fp32, bf16 or fp16, got {x.dtype}")
-    if log_decay.dtype != x.dtype and log_decay.dtype != torch.float32:
+    if g_code != code and g_code != _lib.DTYPE_F32:
         raise TypeError(f"log_decay must be {x.dtype} or fp32, got {log_decay.dtype}")
-    if not x.is_cuda or log_decay.device != x.device:
+    index = x.get_device()
+    if index < 0 or log_decay.get_device() != index:
         raise ValueError(f"{what} and log_decay must be CUDA tensors on one device")
-    _lib.require_device(x, what)
+    index = _lib.device_index(x, what)
     lead = 2 if cu_seqlens is None else 1
     shape = x.shape
     dims = len(shape) - lead
@@ -51,18 +51,19 @@ def _layout(x, log_decay, state, cu_seqlens, what):
     if cu_seqlens is None:
         seqs, rows = shape[0], shape[1]
     else:
-        if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.device != x.device:
+        if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.get_device() != index:
             raise ValueError("cu_seqlens must be int32 [sequences + 1] on the device of the rows")
         if cu_seqlens.numel() < 1 or not cu_seqlens.is_contiguous():
             raise ValueError("cu_seqlens must be contiguous and hold at least one offset")
         seqs, rows = cu_seqlens.numel() - 1, shape[0]
+    state_shape = (seqs, *shape[lead:])
     if state is not None:
-        _check_state(state, x, (seqs, *shape[lead:]), "state")
-    return lead, seqs, rows, heads, d, shared
+        _check_state(state, index, state_shape, "state")
+    return index, code, g_code, lead, seqs, rows, heads, d, shared, state_shape
 
 
-def _check_state(state, x, shape, name):
-    if state.dtype != torch.float32 or state.device != x.device:
+def _check_state(state, index, shape, name):
+    if state.dtype != torch.float32 or state.get_device() != index:
         raise TypeError(f"{name} must be fp32 on the device of the rows")
     if state.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(state.shape)}")
@@ -88,18 +89,20 @@ def _rows(t, lead, channels):
 
 
 def _forward(x, log_decay, state, cu_seqlens, reverse, out, out_state):
-    lead, seqs, rows, heads, d, shared = _layout(x, log_decay, state, cu_seqlens, "x")
-    shape, device, channels = (seqs, *x.shape[lead:]), x.device, heads * d
-    y = torch.empty(x.shape, dtype=x.dtype, device=device) if out is None else out
-    if out is not None:
-        if out.shape != x.shape or out.dtype != x.dtype or out.device != device:
+    index, code, g_code, lead, seqs, rows, heads, d, shared, shape = _layout(x, log_decay, state, cu_seqlens, "x")
+    device, channels = x.device, heads * d
+    if out is None:
+        y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    else:
+        y = out
+        if out.shape != x.shape or out.dtype != x.dtype or out.get_device() != index:
             raise ValueError("out must match x in shape, dtype and device")
         if _rows(out, lead, channels)[0] is not out:
             raise ValueError("out's channels must be contiguous")
     if out_state is None:
         out_state = torch.empty(shape, dtype=torch.float32, device=device)
     else:
-        _check_state(out_state, x, shape, "out_state")
+        _check_state(out_state, index, shape, "out_state")
         if not out_state.is_contiguous():
             raise ValueError("out_state must be contiguous")
     if channels == 0:
@@ -109,11 +112,12 @@ def _forward(x, log_decay, state, cu_seqlens, reverse, out, out_state):
     x, x_batch, x_row = _rows(x, lead, channels)
     log_decay, g_batch, g_row = _rows(log_decay, lead, heads if shared else channels)
     _, y_batch, y_row = _rows(y, lead, channels)
-    state = None if state is None else state.contiguous()
-    _lib.call_on(device, "vdn_gated_scan", x.data_ptr(), _lib.dtype_code(x.dtype), x_batch, x_row,
-                 log_decay.data_ptr(), _lib.dtype_code(log_decay.dtype), g_batch, g_row, shared, _lib.address(state),
-                 _lib.address(cu_seqlens), seqs, rows, heads, d, reverse, y.data_ptr(), y_batch, y_row, out is None,
-                 out_state.data_ptr(), status_address(device))
+    if state is not None and not state.is_contiguous():
+        state = state.contiguous()
+    _lib.call_on(index, "vdn_gated_scan", x.data_ptr(), code, x_batch, x_row, log_decay.data_ptr(), g_code, g_batch,
+                 g_row, shared, None if state is None else state.data_ptr(),
+                 None if cu_seqlens is None else cu_seqlens.data_ptr(), seqs, rows, heads, d, reverse, y.data_ptr(),
+                 y_batch, y_row, out is None, out_state.data_ptr(), status_address(device))
     return y, out_state
 
 
@@ -158,19 +162,24 @@ def gated_scan(x, log_decay, state=None, *, cu_seqlens=None, reverse=False, out=
     return _forward(x, log_decay, state, cu_seqlens, bool(reverse), out, out_state)
 
 
-@torch.no_grad()
 def gated_scan_backward(grad_y, log_decay, y, *, state=None, grad_state=None, cu_seqlens=None, reverse=False):
     """(grad of x, of log_decay, of state) from the forward's output y and its arguments.
 
     grad_state is the gradient of the last state, if any; the gradient of the first state
     comes back as fp32 also when `state` was None.  Rows behind the last packed sequence
-    have zero gradients."""
-    lead, seqs, rows, heads, d, shared = _layout(y, log_decay, state, cu_seqlens, "y")
-    if grad_y.shape != y.shape or grad_y.dtype != y.dtype or grad_y.device != y.device:
+    have zero gradients.  Records nothing for autograd."""
+    if torch.is_grad_enabled():
+        with torch.no_grad():
+            return _backward(grad_y, log_decay, y, state, grad_state, cu_seqlens, bool(reverse))
+    return _backward(grad_y, log_decay, y, state, grad_state, cu_seqlens, bool(reverse))
+
+
+def _backward(grad_y, log_decay, y, state, grad_state, cu_seqlens, reverse):
+    index, code, g_code, lead, seqs, rows, heads, d, shared, shape = _layout(y, log_decay, state, cu_seqlens, "y")
+    if grad_y.shape != y.shape or grad_y.dtype != y.dtype or grad_y.get_device() != index:
         raise ValueError("grad_y must match y in shape, dtype and device")
-    shape = (seqs, *y.shape[lead:])
     if grad_state is not None:
-        _check_state(grad_state, y, shape, "grad_state")
+        _check_state(grad_state, index, shape, "grad_state")
         grad_state = grad_state.contiguous()
     device, channels = y.device, heads * d
     dx = torch.empty(y.shape, dtype=y.dtype, device=device)
@@ -184,10 +193,11 @@ def gated_scan_backward(grad_y, log_decay, y, *, state=None, grad_state=None, cu
     y, y_batch, y_row = _rows(y, lead, channels)
     _, dx_batch, dx_row = _rows(dx, lead, channels)
     _, dg_batch, dg_row = _rows(dg, lead, decays)
-    state = None if state is None else state.contiguous()
-    _lib.call_on(device, "vdn_gated_scan_backward", grad_y.data_ptr(), _lib.dtype_code(y.dtype), dy_batch, dy_row,
-                 log_decay.data_ptr(), _lib.dtype_code(log_decay.dtype), g_batch, g_row, shared, y.data_ptr(), y_batch,
-                 y_row, _lib.address(state), _lib.address(grad_state), _lib.address(cu_seqlens), seqs, rows, heads, d,
-                 bool(reverse), dx.data_ptr(), dx_batch, dx_row, dg.data_ptr(), dg_batch, dg_row, True,
-                 ds.data_ptr(), status_address(device))
+    if state is not None and not state.is_contiguous():
+        state = state.contiguous()
+    _lib.call_on(index, "vdn_gated_scan_backward", grad_y.data_ptr(), code, dy_batch, dy_row, log_decay.data_ptr(),
+                 g_code, g_batch, g_row, shared, y.data_ptr(), y_batch, y_row, None if state is None else state.data_ptr(),
+                 None if grad_state is None else grad_state.data_ptr(),
+                 None if cu_seqlens is None else cu_seqlens.data_ptr(), seqs, rows, heads, d, reverse, dx.data_ptr(),
+                 dx_batch, dx_row, dg.data_ptr(), dg_batch, dg_row, True, ds.data_ptr(), status_address(device))
     return dx, dg, ds
