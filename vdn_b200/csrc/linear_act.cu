@@ -796,7 +796,8 @@ static int run_pair(const Operand& x, const Operand& f, int64_t depth, Params p,
 }
 
 template <typename T, bool F_MN, bool X_MN, int ACT, int BN>
-static int run_narrow(const Operand& x, const Operand& f, int64_t depth, Params p, const Dev& d, cudaStream_t stream) {
+static int run_narrow(const Operand& x, const Operand& f, int64_t depth, Params p, const Dev& d, int split,
+                      cudaStream_t stream) {
   CUtensorMap mf, mx;
   if (int rc = F_MN ? operand_map<T>(&mf, f.base, p.cols, depth, f.ld, true, 0)
                     : operand_map<T>(&mf, f.base, depth, p.cols, f.ld, false, 128)) return rc;
@@ -805,10 +806,6 @@ static int run_narrow(const Operand& x, const Operand& f, int64_t depth, Params 
   p.m_tiles = (int)((p.cols + 127) / 128);
   p.n_tiles = (int)((p.rows + BN - 1) / BN);
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
-  // Two CTAs fit an SM: split the depth while that leaves a fifth of the places free (clusters
-  // of eight do not pack into every GPC: a second wave cost 6 us of 11) and each CTA four blocks.
-  int split = 1;
-  while (split < 8 && tiles * split * 2 * 5 <= 2 * d.sms * 4 && p.k_blocks >= 8 * split) split *= 2;
   auto* kernel = narrow_kernel<T, F_MN, X_MN, ACT, BN>;
   VDN_ALLOW_SMEM(kernel, narrow_smem<BN>(), d.index);
   VDN_CHECK_ARG(tiles * split < (1ll << 31), "too many tiles for one launch");
@@ -827,6 +824,28 @@ static int run_narrow(const Operand& x, const Operand& f, int64_t depth, Params 
   return VDN_OK;
 }
 
+// Tokens a tile and CTAs that split the depth.  In units of 10 ns, measured: a CTA costs 300 to
+// start, 10 + BN / 8 a depth block (its bytes through L2), 6 a token of epilogue; a split
+// shares the epilogue but adds 250 for its two cluster barriers.  Two CTAs fit an SM; clusters
+// take four fifths of the places at most (those of eight do not pack into every GPC: a second
+// wave cost 6 us of 11).
+static void narrow_shape(int64_t rows, int64_t cols, int k_blocks, int least, int sms, int& bn, int& split) {
+  int64_t best = -1;
+  for (int b = least; b <= 128; b *= 2) {
+    const int64_t tiles = ((cols + 127) / 128) * ((rows + b - 1) / b);
+    for (int s = 1; s <= 8; s *= 2) {
+      if (s > 1 && (tiles * s * 5 > 2 * sms * 4 || k_blocks < 2 * s)) break;
+      const int64_t waves = (tiles * s + 2 * sms - 1) / (2 * sms), share = tiles * s > sms ? 2 : 1;
+      const int64_t t = waves * (300 + share * ((int64_t)(k_blocks + s - 1) / s * (10 + b / 8) + 6 * b / s) + (s > 1 ? 250 + b : 0));
+      if (best < 0 || t < best) {
+        best = t;
+        bn = b;
+        split = s;
+      }
+    }
+  }
+}
+
 // y [rows, cols] = sum over depth of x[rows] f[cols].
 template <typename T, bool X_MN, bool F_MN, int ACT>
 static int product(const Operand& x, const Operand& f, int64_t depth, Params p, cudaStream_t stream) {
@@ -838,28 +857,44 @@ static int product(const Operand& x, const Operand& f, int64_t depth, Params p, 
   // SMs without work; narrow tiles with a split depth fill them.
   VDN_CHECK_ARG(pair_tiles < (1ll << 29), "too many tiles for one launch");
   if (pair_tiles >= 28 && p.rows > 128) return run_pair<T, X_MN, F_MN, ACT>(x, f, depth, p, d, stream);
+  int bn = 128, split = 1;
+  narrow_shape(p.rows, p.cols, p.k_blocks, X_MN ? 64 : 16, d.sms, bn, split);
   if constexpr (!X_MN) {
-    if (p.rows <= 16) return run_narrow<T, F_MN, X_MN, ACT, 16>(x, f, depth, p, d, stream);
-    if (p.rows <= 32) return run_narrow<T, F_MN, X_MN, ACT, 32>(x, f, depth, p, d, stream);
-    if (p.rows <= 64) return run_narrow<T, F_MN, X_MN, ACT, 64>(x, f, depth, p, d, stream);
+    if (bn == 16) return run_narrow<T, F_MN, X_MN, ACT, 16>(x, f, depth, p, d, split, stream);
+    if (bn == 32) return run_narrow<T, F_MN, X_MN, ACT, 32>(x, f, depth, p, d, split, stream);
   }
-  return run_narrow<T, F_MN, X_MN, ACT, 128>(x, f, depth, p, d, stream);
+  if (bn == 64) return run_narrow<T, F_MN, X_MN, ACT, 64>(x, f, depth, p, d, split, stream);
+  return run_narrow<T, F_MN, X_MN, ACT, 128>(x, f, depth, p, d, split, stream);
 }
 
-// Copies up to two matrices into rows whose stride the tensor maps take (odd depths, unaligned views).
+// Copies up to two matrices into rows whose stride the tensor maps take (odd depths, unaligned
+// views): a thread per 16 bytes written, read in the widest pieces the source's alignment allows.
 struct Pad {
   const uint16_t* src[2];
   uint16_t* dst[2];
   int64_t rows[2], cols[2], ld[2], to[2];
+  int piece[2];          // values a load takes: 4, 2 or 1
 };
 __global__ void __launch_bounds__(256) pad_kernel(const Pad p) {
   const int m = blockIdx.y;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= p.rows[m]) return;
-  const uint16_t* s = p.src[m] + row * p.ld[m];
-  uint16_t* d = p.dst[m] + row * p.to[m];
-#pragma unroll 4
-  for (int64_t c = threadIdx.x & 31; c < p.cols[m]; c += 32) d[c] = s[c];
+  const int64_t per = p.to[m] / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= p.rows[m] * per) return;
+  const int64_t row = i / per, c = (i - row * per) * 8;
+  const uint16_t* s = p.src[m] + row * p.ld[m] + c;
+  const int n = (int)min((int64_t)8, p.cols[m] - c);
+  alignas(16) uint16_t v[8] = {};
+  if (n == 8 && p.piece[m] == 4) {
+    reinterpret_cast<uint2*>(v)[0] = reinterpret_cast<const uint2*>(s)[0];
+    reinterpret_cast<uint2*>(v)[1] = reinterpret_cast<const uint2*>(s)[1];
+  } else if (n == 8 && p.piece[m] == 2) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) reinterpret_cast<uint32_t*>(v)[k] = reinterpret_cast<const uint32_t*>(s)[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < n) v[k] = s[k];
+  }
+  *reinterpret_cast<uint4*>(p.dst[m] + row * p.to[m] + c) = *reinterpret_cast<const uint4*>(v);
 }
 
 static int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
@@ -889,7 +924,9 @@ static int settle(std::initializer_list<Matrix> operands, uint8_t*& ws, size_t& 
     p.cols[n] = o.cols;
     p.ld[n] = o.ld;
     p.to[n] = pad8(o.cols);
-    most = o.rows > most ? o.rows : most;
+    p.piece[n] = o.ld % 4 == 0 && aligned_to(o.base, 8) ? 4 : o.ld % 2 == 0 && aligned_to(o.base, 4) ? 2 : 1;
+    const int64_t vectors = o.rows * (pad8(o.cols) / 8);
+    most = vectors > most ? vectors : most;
     o.base = ws;
     o.ld = pad8(o.cols);
     ws += bytes;
@@ -897,7 +934,7 @@ static int settle(std::initializer_list<Matrix> operands, uint8_t*& ws, size_t& 
     ++n;
   }
   if (!n) return VDN_OK;
-  pad_kernel<<<dim3((unsigned)((most + 7) / 8), n), 256, 0, stream>>>(p);
+  pad_kernel<<<dim3((unsigned)((most + 255) / 256), n), 256, 0, stream>>>(p);
   VDN_LAUNCH_CHECK("linear (padded operands)");
   return VDN_OK;
 }

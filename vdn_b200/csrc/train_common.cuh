@@ -135,34 +135,41 @@ template <typename R> __device__ __forceinline__ void store_once(void* p, const 
 
 inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
-// Sums `lines` lines of `cols` fp32 partial sums in a fixed order: 32 columns by 32 line
-// groups a block.  Columns below `split` go to `a`, the others to `b` (either may be null).
+// Sums `lines` lines of `cols` fp32 partial sums in a fixed order: 8 columns (a 32-byte sector a
+// line) by 128 line groups a block, so that few columns still have many loads in flight.
+// Columns below `split` go to `a`, the others to `b` (either may be null).
 template <typename T>
 __global__ void __launch_bounds__(1024) lines_kernel(const float* part, int lines, int64_t cols, T* a, int64_t split,
                                                      T* b) {
-  __shared__ float sums[32][33];
-  const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  __shared__ float sums[8][129];
+  const int col = threadIdx.x & 7, group = threadIdx.x >> 3;
+  const int64_t c = (int64_t)blockIdx.x * 8 + col;
   float s = 0.f;
   if (c < cols) {
 #pragma unroll 4
-    for (int l = g; l < lines; l += 32) s += part[l * cols + c];
+    for (int l = group; l < lines; l += 128) s += part[l * cols + c];
   }
-  sums[g][lane] = s;
+  sums[col][group] = s;
   __syncthreads();
-  if (g == 0 && c < cols) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;   // a warp per column
+  if (warp >= 8) return;
+  s = sums[warp][lane];
 #pragma unroll
-    for (int k = 1; k < 32; ++k) s += sums[k][lane];
-    if (c < split) {
-      if (a) a[c] = from_f32<T>(s);
+  for (int k = 32; k < 128; k += 32) s += sums[warp][lane + k];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int64_t at = (int64_t)blockIdx.x * 8 + warp;
+  if (lane == 0 && at < cols) {
+    if (at < split) {
+      if (a) a[at] = from_f32<T>(s);
     } else if (b) {
-      b[c - split] = from_f32<T>(s);
+      b[at - split] = from_f32<T>(s);
     }
   }
 }
 template <typename T>
 inline int add_lines(const float* part, int lines, int64_t cols, T* a, int64_t split, T* b, cudaStream_t stream) {
-  lines_kernel<T><<<(unsigned)((cols + 31) / 32), 1024, 0, stream>>>(part, lines, cols, a, split, b);
+  lines_kernel<T><<<(unsigned)((cols + 7) / 8), 1024, 0, stream>>>(part, lines, cols, a, split, b);
   VDN_LAUNCH_CHECK("line sums");
   return VDN_OK;
 }
