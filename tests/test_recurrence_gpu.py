@@ -239,24 +239,28 @@ def test_rows_outside_the_sequences_do_not_matter(cuda, shared, reverse):
 
 
 def test_offsets_past_32_bits(cuda):
-    """2.2e9 elements: the last rows equal a scan of their own from the state before them."""
+    """2.2e9 elements: the last rows equal a scan of their own from the state before them.  The two
+    group the sums differently, so each side errs by 8u E (|x| < 5, decay 0.78: M < 23, E < 105:
+    5e-5) before its own rounding to bf16 by 2^-8 of the value: 2^-7 |value| + 1e-4 apart at most.
+    In the backward |h| < 23 multiplies the fp32 part for dg."""
     from vdn_b200.recurrence import gated_scan, gated_scan_backward
     n, c, tail = 430000, 5120, 64
     x = torch.zeros(1, n, c, dtype=torch.bfloat16, device=cuda)
     g = torch.full((1, n, c), -0.25, dtype=torch.bfloat16, device=cuda)
     gen = torch.Generator(device=cuda).manual_seed(1)
-    x[:, -tail:] = torch.randn(1, tail, c, generator=gen, device=cuda).bfloat16()
+    x[:, -tail:] = torch.randn(1, tail, c, generator=gen, device=cuda).clamp(-5, 5).bfloat16()
     y, last = gated_scan(x, g)
     want, wlast = gated_scan(x[:, -tail:].contiguous(), g[:, -tail:].contiguous())
     assert not bool(y[:, :-tail].any())
-    err = 2.0 ** -8 * want.float().abs() + 1e-5
-    assert bool(((y[:, -tail:].float() - want.float()).abs() <= err).all())
+    near = lambda a, b, fp32: bool(((a.float() - b.float()).abs() <= 2.0 ** -7 * b.float().abs() + fp32).all())
+    assert near(y[:, -tail:], want, 1e-4)
     assert float((last - wlast).abs().max()) < 1e-4
-    del x
-    dx, dg, _ = gated_scan_backward(y, g, y)
-    wx, wg, _ = gated_scan_backward(want, g[:, -tail:].contiguous(), want)
-    for a, b in ((dx, wx), (dg, wg)):
-        assert bool(((a[:, -tail:].float() - b.float()).abs() <= 2.0 ** -6 * b.float().abs() + 1e-3).all())
+    grad = x
+    grad[:, -tail:] = torch.randn(1, tail, c, generator=gen, device=cuda).clamp(-5, 5).bfloat16()
+    y[:, -tail:] = want
+    dx, dg, _ = gated_scan_backward(grad, g, y)
+    wx, wg, _ = gated_scan_backward(grad[:, -tail:].contiguous(), g[:, -tail:].contiguous(), want)
+    assert near(dx[:, -tail:], wx, 1e-4) and near(dg[:, -tail:], wg, 23e-4)
 
 
 def test_steps_continue_a_scan(cuda):

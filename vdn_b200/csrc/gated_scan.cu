@@ -43,9 +43,6 @@ namespace gscan {
 using namespace sm100;
 
 constexpr int MAX_CLUSTER = 8;
-// Warps a CTA, at most: the backward per channel keeps the most tiles, so that eight warps would
-// leave one CTA an SM (480 us against 327 on the clip).
-template <bool BWD, bool SHARED> constexpr int max_warps() { return BWD && !SHARED ? 4 : 8; }
 
 struct Params {
   const void* x;        // forward: x; backward: dy
@@ -169,11 +166,30 @@ constexpr int tile_bytes() {   // of one warp and stage: x (dy), the saved y, th
   return 32 * VEC * L * ((BWD ? 2 : 1) * (int)sizeof(T) + (SHARED ? 0 : (int)sizeof(TG)));
 }
 
+// Tokens a warp.  Runs of 32 keep all their arrays in up to 255 registers and halve the rounds,
+// each of which costs a warp some 250 instructions beside its tokens'; runs of 16 leave room
+// for more warps.  The same whatever the alignment, so that strides do not change the order of
+// the sums.
+constexpr int kRun = 16, kLongRun = 32;
+
+// Warps a CTA, at most.  Runs of 16: the backward per channel keeps the most tiles, so that
+// eight warps would leave one CTA an SM (480 us against 327 on a 1 x 32760 x 5120 backward).
+// Runs of 32: as many as fit the shared memory beside the kernel's fixed arrays.
+template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED>
+constexpr int max_warps() {
+  if (L < kLongRun) return BWD && !SHARED ? 4 : 8;
+  constexpr int line = Lanes<VEC>::N * 32 * (int)sizeof(Fold<typename Lanes<VEC>::V>);
+  int w = 8;   // folds of two rounds, of the cluster's CTAs, and sums
+  while (w > 1 && w * kStages * tile_bytes<T, TG, VEC, L, BWD, SHARED>() + (3 * w + 2 * MAX_CLUSTER) * line + 1024 > 227 * 1024)
+    w /= 2;
+  return w;
+}
+
 template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED, int FROM>
-__global__ void __launch_bounds__(max_warps<BWD, SHARED>() * 32, BWD && !SHARED ? 3 : 2)
+__global__ void __launch_bounds__(max_warps<T, TG, VEC, L, BWD, SHARED>() * 32, L == kLongRun ? 1 : BWD && !SHARED ? 3 : 2)
     scan_kernel(const Params p, const int cluster, const __grid_constant__ Maps maps) {
   constexpr int GV = SHARED ? 1 : VEC;               // decays per lane and token
-  constexpr int TILE = 32 * VEC, MAX_WARPS = max_warps<BWD, SHARED>();
+  constexpr int TILE = 32 * VEC, MAX_WARPS = max_warps<T, TG, VEC, L, BWD, SHARED>();
   constexpr bool RING = FROM != ROWS_LOAD;
   using RX = Raw<T, VEC>;
   using RG = Raw<TG, GV>;
@@ -521,6 +537,7 @@ __global__ void __launch_bounds__(max_warps<BWD, SHARED>() * 32, BWD && !SHARED 
       // Sum each token's terms over the head: the first rounds halve the tokens a lane
       // holds while they halve the lanes, so L sums cost about L + 5 shuffles.
       if (n > 0) {
+        constexpr int per = 32 / L;                  // lanes that end with parts of one token
         int off = 16;
 #pragma unroll
         for (int m = L; m > 1; m >>= 1, off >>= 1) {
@@ -532,7 +549,6 @@ __global__ void __launch_bounds__(max_warps<BWD, SHARED>() * 32, BWD && !SHARED 
           }
         }
         float total = dgs[0];
-        const int per = 2 * off;                     // lanes that hold parts of one token
         for (; off; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
         if (lane % per == 0 && lane / per < n) qdg[lane / per * sdg] = from_f32<TG>(total);
       }
@@ -633,8 +649,8 @@ static int prepare(int& dev) {
   VDN_CUDA_TRY(cudaGetDevice(&dev));
   VDN_CHECK_ARG(dev >= 0 && dev < kDevices, "device index out of range");
   if (bytes && !set[dev]) {
-    VDN_CUDA_TRY(cudaFuncSetAttribute(scan_kernel<T, TG, VEC, L, BWD, SHARED, FROM>,
-                                      cudaFuncAttributeMaxDynamicSharedMemorySize, max_warps<BWD, SHARED>() * bytes));
+    VDN_CUDA_TRY(cudaFuncSetAttribute(scan_kernel<T, TG, VEC, L, BWD, SHARED, FROM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      max_warps<T, TG, VEC, L, BWD, SHARED>() * bytes));
     set[dev] = true;
   }
   return VDN_OK;
@@ -655,25 +671,28 @@ static void configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, int64_
 }
 
 // Warps a CTA and CTAs a cluster.  More CTAs on a sequence shorten its walk, but a grid that does
-// not fit the GPU at once runs in waves, the last perhaps nearly empty (the clip's 80 tiles:
-// 305 us with clusters of 8, which need 640 places where there are 592, and 282 us with 5),
-// and every CTA starts up anew.  Measured over clusters of one to eight, CTAs of four and
-// eight warps and nine shapes, a round takes about as long as 1 + (the warps on the fullest SM)
-// / 4 (shared decays, which cost one evaluation per token instead of one per element: 2 + ..),
-// and starting up as two rounds; choosing by that was within a tenth of the best of them.  The ring kernel's places decide for both kernels, so that the order of the sums does
-// not hang on alignment.
+// not fit the GPU at once runs in waves, the last perhaps nearly empty (80 tiles of 32760 tokens,
+// four warps a CTA and 16 tokens a warp: 305 us with clusters of 8, which need 640 places where
+// there are 592, and 282 us with 5), and every CTA starts up anew.  Measured over clusters of one
+// to eight, CTAs of two, four and eight warps and nine shapes, a round takes about as long as
+// 1 + (the warps on the fullest SM) / 4, and starting up as two rounds; choosing by that was
+// within a tenth of the best of them.  Shared decays cost one evaluation per token instead of
+// one per element: 2 + .. / 4.  Runs of 32 take (2 + the warps) / 4, each scheduler's warps
+// counting as its fullest one's, and no less than 6 / 4: a CTA of six warps on four schedulers
+// takes eight warps' time.  The ring kernel's places decide for both kernels, so that the order
+// of the sums does not hang on alignment.
 template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED>
 static int choose_shape(int64_t mean, int64_t longest, int64_t seqs, int64_t tiles, int& warps, int& cluster) {
-  constexpr int FROM = VEC > 1 || SHARED ? ROWS_UP : ROWS_LOAD, MAX_WARPS = max_warps<BWD, SHARED>();
+  constexpr int FROM = VEC > 1 || SHARED ? ROWS_UP : ROWS_LOAD;
   static int places[kDevices][4][MAX_CLUSTER + 1] = {};
   int dev = 0;
   if (int rc = prepare<T, TG, VEC, L, BWD, SHARED, FROM>(dev)) return rc;
-  warps = pow2_at_least<MAX_WARPS>((longest + L - 1) / L);
+  warps = pow2_at_least<max_warps<T, TG, VEC, L, BWD, SHARED>()>((longest + L - 1) / L);
   cluster = 1;
   const int64_t ids = seqs * tiles;
   int64_t best = -1;
-  const int most = warps;                            // fewer warps only from eight to four
-  for (int w = most; w == most || w >= 4; w /= 2) {
+  const int most = warps;
+  for (int w = most; w == most || w >= (L == kLongRun ? 2 : 4); w /= 2) {
     const int64_t runs = (mean + w * L - 1) / (w * L), most_runs = (longest + w * L - 1) / (w * L);
     for (int c = 1; c <= MAX_CLUSTER && c <= (most_runs > 1 ? most_runs : 1); ++c) {
       int& fit = places[dev][w == 8 ? 3 : w >> 1][c];   // clusters resident at once
@@ -686,7 +705,12 @@ static int choose_shape(int64_t mean, int64_t longest, int64_t seqs, int64_t til
         fit = n > 0 ? n : 1;
       }
       const int64_t waves = (ids + fit - 1) / fit, tail = ids - (waves - 1) * fit;
-      auto load = [&](int64_t clusters) { return (SHARED ? 8 : 4) + w * ((clusters * c + 147) / 148); };
+      auto load = [&](int64_t clusters) {
+        const int64_t on_sm = w * ((clusters * c + 147) / 148);
+        if (L < kLongRun) return (SHARED ? 8 : 4) + on_sm;
+        const int64_t t = 2 + (on_sm + 3) / 4 * 4;
+        return t > 6 ? t : 6;
+      };
       // the longest sequences' tiles go on alone
       const int64_t t = ((runs + c - 1) / c + 2) * ((waves - 1) * load(fit) + load(tail)) +
                         ((most_runs + c - 1) / c - (runs + c - 1) / c) * load(tiles);
@@ -714,11 +738,15 @@ static int launch_from(const Params& p, int warps, int cluster, const Maps& maps
   return VDN_OK;
 }
 
+static int64_t mean_length(const Params& p) {
+  return p.cu ? (p.rows + p.seqs - 1) / p.seqs : (int64_t)p.rows;
+}
+
 template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED>
 static int launch(const Params& p, cudaStream_t stream) {
   // A packed batch's lengths live on the device.  Their mean stands for most of them, and random
   // cuts make the longest about 1 + ln(sequences) times as long.
-  const int64_t len = p.cu ? (p.rows + p.seqs - 1) / p.seqs : (int64_t)p.rows;
+  const int64_t len = mean_length(p);
   int64_t longest = len;
   if (p.cu) {
     for (int64_t s = p.seqs; s > 1; s /= 2) longest += len * 7 / 10;
@@ -781,21 +809,26 @@ static int dispatch(Params& p, int shared_dim, cudaStream_t stream) {
     VDN_LAUNCH_CHECK("gated scan step");
     return VDN_OK;
   }
-  // Tokens a warp: as many as its registers hold (the backward keeps twice the arrays),
-  // the same whatever the alignment, so that strides do not change the order of the sums.
-  constexpr int L = 16;
   if (shared_dim) {                                  // one head per tile
     const int vec = shared_dim / 32;
     VDN_CHECK_ARG(fits(vec), "a shared decay needs rows aligned to %d elements", vec);
     p.tiles = (int)(p.channels / shared_dim);
-    if (vec == 4) return launch<T, TG, 4, L / 2, BWD, true>(p, stream);
-    if (vec == 2) return launch<T, TG, 2, L, BWD, true>(p, stream);
-    return launch<T, TG, 1, L, BWD, true>(p, stream);
+    if (vec == 4) return launch<T, TG, 4, kRun / 2, BWD, true>(p, stream);
+    if (vec == 2) return launch<T, TG, 2, kRun, BWD, true>(p, stream);
+    return launch<T, TG, 1, kRun, BWD, true>(p, stream);
   }
   const int vec = fits(2) ? 2 : 1;
   p.tiles = (int)((p.channels + 32 * vec - 1) / (32 * vec));
-  if (vec == 2) return launch<T, TG, 2, L, BWD, false>(p, stream);
-  return launch<T, TG, 1, L, BWD, false>(p, stream);
+  // Long runs where tiles are few and sequences long, so that a round's latency counts and not
+  // the number of warps: us with 16 and 32 tokens a warp, 16-bit rows of 1 x 16384 x 512 (8 tiles)
+  // 46 and 34 (backward 71 and 41), 1 x 32760 x 5120 (80) 288 and 272 (327 and 348), 64 x 512 x
+  // 5120 (5120) 223 and 233 (317 and 390), 2 x 500 x 512 (16) 8 and 8 (8 and 10).  Widths that
+  // tensor maps cannot take keep to 16 (3 x 1001 x 515 in fp32: 13 and 21, 19 and 29).
+  const bool few = p.seqs * ((p.channels + 63) / 64) <= (BWD ? 37 : 148) && mean_length(p) >= 1024 && p.channels % 8 == 0;
+  if (vec == 2 && few) return launch<T, TG, 2, kLongRun, BWD, false>(p, stream);
+  if (vec == 2) return launch<T, TG, 2, kRun, BWD, false>(p, stream);
+  if (few) return launch<T, TG, 1, kLongRun, BWD, false>(p, stream);
+  return launch<T, TG, 1, kRun, BWD, false>(p, stream);
 }
 
 template <bool BWD>
