@@ -160,6 +160,51 @@ def test_packed_lengths(cuda, cu, shared, reverse):
 
 
 @pytest.mark.parametrize("dtype,g_dtype", TYPES)
+@pytest.mark.parametrize("tokens,reverse", [(1024, False), (1025, True), (1499, False)])
+def test_long_runs(cuda, dtype, g_dtype, tokens, reverse):
+    """Few tiles and long sequences take 32 tokens a warp: whole and ragged last runs, sharp decays."""
+    gen, x, g = _case(tokens, (1, tokens), 2, 36, dtype, g_dtype, False, sharp=True)
+    _run(cuda, x, g, None, reverse, True, gen)
+
+
+def test_long_runs_packed_and_strided(cuda):
+    from vdn_b200.recurrence import gated_scan, gated_scan_backward
+    gen, x, g = _case(31, (4200,), 1, 64, torch.bfloat16, torch.bfloat16, False)
+    _run(cuda, x, g, [0, 1, 1100, 1100, 4100], True, True, gen)
+    x, g = x[:, 0].to(cuda), g[:, 0].to(cuda)
+    y, last = gated_scan(x[None], g[None])
+    back = gated_scan_backward(x[None], g[None], y)
+    buf = torch.zeros(4200, 3, 66, dtype=torch.bfloat16, device=cuda)   # pairs aligned, tiles not
+    buf[:, 0, 2:], buf[:, 1, 2:], buf[:, 2, 2:] = x, g, y[0]
+    xs, gs, ys = (buf[:, i, 2:][None] for i in range(3))
+    for a, b in zip((*gated_scan(xs, gs), *gated_scan_backward(xs, gs, ys)), (y, last, *back)):
+        assert torch.equal(a, b)
+    buf = torch.zeros(4200, 3, 67, dtype=torch.bfloat16, device=cuda)   # odd rows: single channels a lane
+    buf[:, 0, 1:65], buf[:, 1, 1:65], buf[:, 2, 1:65] = x, g, y[0]
+    xs, gs, ys = (buf[:, i, 1:65][None] for i in range(3))
+    flat = lambda t: t.double().cpu()
+    zero = torch.zeros(64, dtype=torch.float64)
+    ref = _reference(flat(x), flat(g), zero, flat(x), zero, flat(y[0]))
+    half = _half(torch.bfloat16)
+    dx, dg, _ = gated_scan_backward(xs, gs, ys)
+    for name, got in (("y", gated_scan(xs, gs)[0]), ("dx", dx), ("dg", dg)):
+        _close(got[0], ref[name], ref[name + "_err"] + half * (ref[name].abs() + ref[name + "_err"]) + 2.0 ** -134, name)
+
+
+@pytest.mark.parametrize("seqs", [2, 31, 32, 33])
+def test_packed_order(cuda, seqs):
+    """Up to 32 packed sequences start longest first: equal lengths, empty ones, the longest last."""
+    lengths = [(7 * i) % 5 * 3 for i in range(seqs - 1)] + [90]
+    cu = [2]
+    for n in lengths:
+        cu.append(cu[-1] + n)
+    gen, x, g = _case(seqs, (cu[-1] + 5,), 1, 64, torch.bfloat16, torch.float32, False)
+    y, (dx, dg, _) = _run(cuda, x, g, cu, False, True, gen)
+    for t in (y, dx, dg):
+        assert bool((t[cu[-1]:] == 0).all())
+
+
+@pytest.mark.parametrize("dtype,g_dtype", TYPES)
 def test_restarts_and_strong_decays(cuda, dtype, g_dtype):
     """log_decay = -inf starts a channel anew, next to decays close to 1."""
     gen, x, g = _case(11, (1, 500), 2, 48, dtype, g_dtype, False, sharp=True)

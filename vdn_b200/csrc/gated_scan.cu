@@ -185,6 +185,22 @@ constexpr int max_warps() {
   return w;
 }
 
+// Packed sequences start longest first, so that more CTAs a sequence pay although they do not all
+// fit the GPU at once (7 random cuts of 16389 x 5120 backward, shared decays: 205 us as one wave
+// of clusters of two, 150 as three waves of clusters of three).  The turn-th longest; each
+// lane ranks one, hence at most 32.
+constexpr int kSorted = 32;
+__device__ __forceinline__ int longest_first(const Params& p, int turn, int lane) {
+  const int seqs = (int)p.seqs;
+  int len = -1, place = 0;
+  if (lane < seqs) len = max(min(p.cu[lane + 1], p.rows) - min(max(p.cu[lane], 0), p.rows), 0);
+  for (int j = 0; j < seqs; ++j) {
+    const int other = __shfl_sync(0xffffffffu, len, j);
+    place += other > len || (other == len && j < lane);
+  }
+  return __ffs(__ballot_sync(0xffffffffu, lane < seqs && place == turn)) - 1;
+}
+
 template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED, int FROM>
 __global__ void __launch_bounds__(max_warps<T, TG, VEC, L, BWD, SHARED>() * 32, L == kLongRun ? 1 : BWD && !SHARED ? 3 : 2)
     scan_kernel(const Params p, const int cluster, const __grid_constant__ Maps maps) {
@@ -206,8 +222,9 @@ __global__ void __launch_bounds__(max_warps<T, TG, VEC, L, BWD, SHARED>() * 32, 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int rank = (int)cluster_ctarank();
   const int64_t id = blockIdx.x / cluster;           // sequence-major, channel tiles fastest
-  const int64_t seq = id / p.tiles;
-  const int tile = (int)(id - seq * p.tiles);
+  const int64_t turn = id / p.tiles;
+  const int tile = (int)(id - turn * p.tiles);
+  const int64_t seq = p.cu && p.seqs <= kSorted && turn < p.seqs ? longest_first(p, (int)turn, lane) : turn;
   const int64_t c = (int64_t)tile * TILE + lane * VEC;
   const bool live = c < p.channels;
   const bool whole = (int64_t)(tile + 1) * TILE <= p.channels;
@@ -682,7 +699,7 @@ static void configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, int64_
 // takes eight warps' time.  The ring kernel's places decide for both kernels, so that the order
 // of the sums does not hang on alignment.
 template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED>
-static int choose_shape(int64_t mean, int64_t longest, int64_t seqs, int64_t tiles, int& warps, int& cluster) {
+static int choose_shape(int64_t mean, int64_t longest, int64_t seqs, bool sorted, int64_t tiles, int& warps, int& cluster) {
   constexpr int FROM = VEC > 1 || SHARED ? ROWS_UP : ROWS_LOAD;
   static int places[kDevices][4][MAX_CLUSTER + 1] = {};
   int dev = 0;
@@ -711,9 +728,15 @@ static int choose_shape(int64_t mean, int64_t longest, int64_t seqs, int64_t til
         const int64_t t = 2 + (on_sm + 3) / 4 * 4;
         return t > 6 ? t : 6;
       };
-      // the longest sequences' tiles go on alone
-      const int64_t t = ((runs + c - 1) / c + 2) * ((waves - 1) * load(fit) + load(tail)) +
-                        ((most_runs + c - 1) / c - (runs + c - 1) / c) * load(tiles);
+      const int64_t walk = (runs + c - 1) / c, longest_walk = (most_runs + c - 1) / c;
+      int64_t t = (walk + 2) * ((waves - 1) * load(fit) + load(tail));
+      if (sorted && waves > 1) {                     // the longest start first, the others fill the places behind
+        const int64_t first = (longest_walk + 2) * load(fit);
+        t = (walk + 2) * load(fit) * ids / fit;
+        if (t < first) t = first;
+      } else {
+        t += (longest_walk - walk) * load(tiles);    // the longest sequences' tiles go on alone
+      }
       if (best < 0 || t < best) {
         best = t;
         warps = w;
@@ -745,15 +768,15 @@ static int64_t mean_length(const Params& p) {
 template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED>
 static int launch(const Params& p, cudaStream_t stream) {
   // A packed batch's lengths live on the device.  Their mean stands for most of them, and random
-  // cuts make the longest about 1 + ln(sequences) times as long.
+  // cuts make the longest somewhat above 1 + ln(sequences) times as long.
   const int64_t len = mean_length(p);
   int64_t longest = len;
   if (p.cu) {
-    for (int64_t s = p.seqs; s > 1; s /= 2) longest += len * 7 / 10;
+    for (int64_t s = p.seqs; s > 1; s /= 2) longest += len * 17 / 20;
     if (longest > p.rows) longest = p.rows;
   }
   int warps = 1, cluster = 1;
-  if (int rc = choose_shape<T, TG, VEC, L, BWD, SHARED>(len, longest, p.seqs, p.tiles, warps, cluster)) return rc;
+  if (int rc = choose_shape<T, TG, VEC, L, BWD, SHARED>(len, longest, p.seqs, p.cu && p.seqs <= kSorted, p.tiles, warps, cluster)) return rc;
   Maps maps = {};
   // Tiles of whole runs pay from two runs a sequence on; shorter ones would mostly copy others' rows.
   if constexpr (VEC > 1 || SHARED) {
