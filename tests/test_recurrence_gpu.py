@@ -201,7 +201,28 @@ def test_packed_order(cuda, seqs):
     gen, x, g = _case(seqs, (cu[-1] + 5,), 1, 64, torch.bfloat16, torch.float32, False)
     y, (dx, dg, _) = _run(cuda, x, g, cu, False, True, gen)
     for t in (y, dx, dg):
-        assert bool((t[cu[-1]:] == 0).all())
+        assert bool((t[cu[-1]:] == 0).all()) and bool((t[:cu[0]] == 0).all())
+
+
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("cu", [[300, 300], [40, 90, 300], [-5, 17, 900]])
+def test_rows_outside_the_sequences_come_back_zero(cuda, shared, cu):
+    """In front of the first sequence as behind the last; offsets out of range are cut off."""
+    from vdn_b200.recurrence import gated_scan, gated_scan_backward
+    gen, x, g = _case(41, (420,), 2, 64, torch.bfloat16, torch.float32, shared)
+    x, g = x.to(cuda), g.to(cuda)
+    cud = torch.tensor(cu, dtype=torch.int32, device=cuda)
+    for _ in range(2):                                       # the second time over memory that held NaN
+        y, _ = gated_scan(x, g, cu_seqlens=cud)
+        dx, dg, _ = gated_scan_backward(x, g, y, cu_seqlens=cud)
+        for t in (y, dx, dg):
+            for part in (t[:max(cu[0], 0)], t[cu[-1]:]):
+                assert bool((part == 0).all())
+            t.fill_(float("nan"))
+        del y, dx, dg, t, part
+    out = torch.full_like(x, 5.0)
+    gated_scan(x, g, cu_seqlens=cud, out=out)
+    assert bool((out[:max(cu[0], 0)] == 5).all()) and bool((out[cu[-1]:] == 5).all())
 
 
 @pytest.mark.parametrize("dtype,g_dtype", TYPES)

@@ -156,10 +156,6 @@ def records(*tensors) -> bool:
     return False
 
 
-def address(t: torch.Tensor | None):
-    return None if t is None else t.data_ptr()
-
-
 def capturing(device: torch.device) -> bool:
     """Whether `device`'s current stream is being captured."""
     if device.type != "cuda":

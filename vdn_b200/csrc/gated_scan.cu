@@ -237,8 +237,10 @@ __global__ void __launch_bounds__(max_warps<T, TG, VEC, L, BWD, SHARED>() * 32, 
     begin = min(max(lo, 0), p.rows);                 // offsets out of range stay inside the tensors
     len = max(min(hi, p.rows) - begin, 0);
   }
-  if (seq >= p.seqs) {                               // rows behind the last sequence
-    for (int64_t t = rank * warps + warp; t < len; t += warps * cluster) {
+  if (seq >= p.seqs) {                               // rows in front of the first sequence and behind the last
+    const int head = min(min(max(p.cu[0], 0), p.rows), begin);
+    for (int64_t i = rank * warps + warp; i < head + len; i += warps * cluster) {
+      const int64_t t = i < head ? i - begin : i - head;
       if (live) *reinterpret_cast<RX*>(static_cast<T*>(p.out) + (begin + t) * p.out_row + c) = raw_zero<RX>();
       if (BWD && (SHARED ? lane == 0 : live))
         *reinterpret_cast<RG*>(static_cast<TG*>(p.dg) + (begin + t) * p.dg_row + gc) = raw_zero<RG>();

@@ -148,8 +148,8 @@ def gated_scan(x, log_decay, state=None, *, cu_seqlens=None, reverse=False, out=
     x [B, T, C] or [B, T, H, d] (fp32, bf16 or fp16); log_decay of x's shape, or [B, T, H]
     for one decay per head (d = 32, 64 or 128), in x's dtype or fp32; -inf restarts a
     channel.  With cu_seqlens (int32 [S + 1] on the device, nondecreasing row offsets) the
-    sequences lie end to end: x [N, C] or [N, H, d]; rows behind the last offset come back
-    zero, and stay as they were in a caller's `out`.  state / out_state fp32 [B or S, C] or
+    sequences lie end to end: x [N, C] or [N, H, d]; rows in front of the first offset and
+    behind the last come back zero, and stay as they were in a caller's `out`.  state / out_state fp32 [B or S, C] or
     [.., H, d]; out_state may be `state` (updated in place).  reverse runs each sequence from
     its last row to its first.  Strided rows and expanded log_decay are read in place as
     long as a row's channels are contiguous.  A state that overflows fp32 comes out as inf or NaN.
@@ -166,7 +166,7 @@ def gated_scan_backward(grad_y, log_decay, y, *, state=None, grad_state=None, cu
     """(grad of x, of log_decay, of state) from the forward's output y and its arguments.
 
     grad_state is the gradient of the last state, if any; the gradient of the first state
-    comes back as fp32 also when `state` was None.  Rows behind the last packed sequence
+    comes back as fp32 also when `state` was None.  Rows outside the packed sequences
     have zero gradients.  Records nothing for autograd."""
     if torch.is_grad_enabled():
         with torch.no_grad():
