@@ -9,7 +9,7 @@
 // per channel and runs join in any grouping.  HBM is the bound: the forward moves three
 // elements per token and channel, the backward five, for a dozen instructions each.  So
 // the inputs are read ONCE and kept in registers while the runs are joined:
-//   * rows travel as tiles (L tokens of a warp's channels) by tensor-map copies, two rounds ahead,
+//   * rows travel as tiles (L tokens of a warp's channels) by tensor-map copies, a round ahead,
 //     and results leave the same way from the tile they replace: no addresses or predicates
 //     per element (with plain loads the scan was bound by issue, half of it such overhead);
 //   * a warp owns L tokens of 32 * VEC channels (lane = VEC neighbouring channels) and folds
@@ -19,9 +19,13 @@
 //   * a cluster of up to eight CTAs owns neighbouring CTA runs and walks the sequence in
 //     rounds.  Each CTA sends its pair into the others' shared memory with asynchronous
 //     stores that count on their mbarriers: unlike a cluster barrier (whose release waits
-//     for the round's output stores: 480 against 355 us below) this orders nothing else.
-//     No flags in global memory, no workspace, and the order of every sum is fixed: the
-//     same bits on every run.
+//     for the round's output stores: 480 against 355 us on an early form of the forward
+//     below) this orders nothing else.  No flags in global memory, no workspace, and the
+//     order of every sum is fixed: the same bits on every run.
+// Measured, 16 bits: 1 x 32760 x 5120 forward 270 us (3.7 TB/s), backward 327 (5.1 TB/s); seven
+// packed sequences of 16389 x 5120 backward, an fp32 decay per head, 145 us (3.5 TB/s).  DRAM
+// and issue slots are half idle: what bounds it is the latency of a round (two walks and the
+// exchange) at the warps that registers and tiles allow.
 //
 // Numerics: states, folds and sums in fp32.  A decay close to 1 loses its distance from
 // 1 when it is rounded to fp32 (a memory of n tokens then errs by n * 2^-25, and a constant decay errs

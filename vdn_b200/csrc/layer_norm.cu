@@ -15,6 +15,8 @@
 // them; one line of partial sums per CTA goes to the caller's workspace, and a second
 // kernel adds the lines in a fixed order.  No atomics: the same bits on every run.
 // Widths that fit no register form take `wide` kernels, which read a row again for each pass.
+// Bound by HBM: 32760 x 5120 in bf16 forward 124 us (5.4 TB/s, a copy reaches 6.5), backward 199
+// (5.1 TB/s, some 10 us of it the sum of the lines).
 #include <initializer_list>
 
 #include "train_common.cuh"

@@ -12,12 +12,14 @@
 //     its 128 rows of P and its 128-row half of Q per 64-deep block (six stages of 32 KB);
 //     the even CTA's MMA warp issues 256 x 256 x 16 products into one of two TMEM
 //     accumulators, so that eight epilogue warps work on a tile while the next one runs.
-//     Bound by the tensor pipe for deep products, by its epilogue for shallow ones.
+//     Bound by the tensor pipe for deep products (32760 x 5120 x 5120: 1123 to 1265 us with
+//     the clocks under load, 1.36 to 1.53 PFLOP/s, as torch's own), by its epilogue for
+//     shallow ones.
 //   * narrow kernel: 128 features x up to 128 tokens per CTA with the features on the MMA's M
 //     side, for outputs too small to fill the GPU with pair tiles (few tokens: the weight's
 //     bytes are the bound).  A cluster of up to eight CTAs splits the sum; the parts meet
 //     through distributed shared memory in rank order.  Lanes are features, so any output
-//     stride is stored coalesced.
+//     stride is stored coalesced.  16 x 13824 x 5120: 31 us, 4.6 TB/s of weight.
 //
 // Rounding: z is rounded once for `pre` and once, after activation and residual in fp32,
 // for y.  dz is rounded to the operand type because the tensor cores take 16 bits; db sums
