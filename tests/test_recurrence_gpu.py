@@ -276,6 +276,28 @@ def test_strides_broadcast_and_outputs(cuda):
     assert torch.equal(gated_scan(x.to(cuda), wide)[0], gated_scan(x.to(cuda), wide.contiguous())[0])
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_shared_decay_of_misaligned_rows(cuda, d):
+    """Rows that start inside a lane's vector are copied; an `out` like that is refused."""
+    from vdn_b200.recurrence import gated_scan, gated_scan_backward
+    gen, x, g = _case(d, (2, 40), 2, d, torch.bfloat16, torch.float32, True)
+    x, g = x.to(cuda), g.to(cuda)
+    y, last = gated_scan(x, g)
+    want = (y, last, *gated_scan_backward(x, g, y))
+    wide = torch.zeros(2, 40, 2 * d + 3, dtype=torch.bfloat16, device=cuda)
+    flat = torch.zeros(x.numel() + 1, dtype=torch.bfloat16, device=cuda)[1:].view(x.shape)   # contiguous
+    for view in (wide[..., 1:2 * d + 1].unflatten(2, (2, d)), flat):
+        def put(t):
+            view.copy_(t)
+            return view
+        got = gated_scan(put(x), g)
+        for a, b in zip((*got, *gated_scan_backward(put(x), g, y), *gated_scan_backward(x, g, put(y))),
+                        (*want, *want[2:])):
+            assert torch.equal(a, b)
+    with pytest.raises(ValueError, match="aligned"):
+        gated_scan(x, g, out=flat)
+
+
 def test_packed_out_keeps_rows_behind_the_last(cuda):
     from vdn_b200.recurrence import gated_scan
     gen, x, g = _case(4, (50,), 2, 32, torch.bfloat16, torch.bfloat16, True)

@@ -88,6 +88,15 @@ def _rows(t, lead, channels):
     return t, channels * shape[1] if shape[0] > 1 else 0, channels if shape[1] > 1 else 0
 
 
+def _aligned(t, batch, row, lead, d):
+    """_rows's result with rows that start at whole vectors of d / 32 values, copied if they do not
+    (a lane of the shared-decay kernels owns that many)."""
+    vec = d // 32
+    if vec > 1 and (batch % vec or row % vec or t.data_ptr() % (vec * t.element_size())):
+        return _rows(t.clone(memory_format=torch.contiguous_format), lead, t.shape[lead:].numel())
+    return t, batch, row
+
+
 def _forward(x, log_decay, state, cu_seqlens, reverse, out, out_state):
     index, code, g_code, lead, seqs, rows, heads, d, shared, shape = _layout(x, log_decay, state, cu_seqlens, "x")
     device, channels = x.device, heads * d
@@ -110,6 +119,8 @@ def _forward(x, log_decay, state, cu_seqlens, reverse, out, out_state):
     if seqs == 0:
         return (y.zero_() if out is None else y), out_state
     x, x_batch, x_row = _rows(x, lead, channels)
+    if shared:
+        x, x_batch, x_row = _aligned(x, x_batch, x_row, lead, d)
     log_decay, g_batch, g_row = _rows(log_decay, lead, heads if shared else channels)
     _, y_batch, y_row = _rows(y, lead, channels)
     if state is not None and not state.is_contiguous():
@@ -191,6 +202,9 @@ def _backward(grad_y, log_decay, y, state, grad_state, cu_seqlens, reverse):
     grad_y, dy_batch, dy_row = _rows(grad_y, lead, channels)
     log_decay, g_batch, g_row = _rows(log_decay, lead, decays)
     y, y_batch, y_row = _rows(y, lead, channels)
+    if shared:
+        grad_y, dy_batch, dy_row = _aligned(grad_y, dy_batch, dy_row, lead, d)
+        y, y_batch, y_row = _aligned(y, y_batch, y_row, lead, d)
     _, dx_batch, dx_row = _rows(dx, lead, channels)
     _, dg_batch, dg_row = _rows(dg, lead, decays)
     if state is not None and not state.is_contiguous():
