@@ -143,7 +143,4 @@ def layer_norm_backward(grad_y, x, weight, mean, rstd, *, bias=True):
     where there is no weight, the bias's unless `bias`.  Parameter gradients come in the
     weight's dtype (x's without one), summed over the rows in fp32 in a fixed order.
     Records nothing for autograd."""
-    if torch.is_grad_enabled():
-        with torch.no_grad():
-            return _backward(grad_y, x, weight, mean, rstd, weight is not None, bool(bias))
     return _backward(grad_y, x, weight, mean, rstd, weight is not None, bool(bias))

@@ -156,7 +156,4 @@ def linear_act_backward(grad_y, x, weight, pre=None, *, act="none", bias=True):
     gradient is grad_y.  The activation's gradient enters the two products rounded to the
     operands' type; the bias gradient sums it unrounded, in fp32 and a fixed order.  Records
     nothing for autograd."""
-    if torch.is_grad_enabled():
-        with torch.no_grad():
-            return _backward(grad_y, x, weight, pre, act, True, True, bool(bias))
     return _backward(grad_y, x, weight, pre, act, True, True, bool(bias))

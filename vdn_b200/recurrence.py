@@ -35,10 +35,10 @@ def _layout(x, log_decay, state, cu_seqlens, what):
         raise ValueError(f"{what} and log_decay must be CUDA tensors on one device")
     index = _lib.device_index(x, what)
     lead = 2 if cu_seqlens is None else 1
-    shape = x.shape
+    shape = tuple(x.shape)
     dims = len(shape) - lead
     if dims == 2:
-        heads, d = shape[-2:]
+        heads, d = shape[-2], shape[-1]
     elif dims == 1:
         heads, d = 1, shape[-1]
     else:
@@ -69,23 +69,28 @@ def _check_state(state, index, shape, name):
         raise ValueError(f"{name} must be {list(shape)}, got {list(state.shape)}")
 
 
+def _dense(shape, lead, channels):
+    """(batch stride, row stride) of a contiguous tensor, as _rows gives them."""
+    if lead == 1:
+        return 0, channels if shape[0] > 1 else 0
+    return channels * shape[1] if shape[0] > 1 else 0, channels if shape[1] > 1 else 0
+
+
 def _rows(t, lead, channels):
     """(t with each row's channels contiguous, copied if they are not; batch stride; row
     stride).  A stride that no index multiplies counts as 0."""
     shape = t.shape
-    if not t.is_contiguous():
-        need = 1
-        for n, s in zip(reversed(shape[lead:]), reversed(t.stride()[lead:])):
-            if n != 1 and s != need:
-                t = t.contiguous()
-                break
-            need *= n
-        stride = t.stride()
-        row = stride[lead - 1] if shape[lead - 1] > 1 else 0
-        return t, (stride[0] if shape[0] > 1 else 0) if lead == 2 else 0, row
-    if lead == 1:
-        return t, 0, channels if shape[0] > 1 else 0
-    return t, channels * shape[1] if shape[0] > 1 else 0, channels if shape[1] > 1 else 0
+    if t.is_contiguous():
+        return t, *_dense(shape, lead, channels)
+    need = 1
+    for n, s in zip(reversed(shape[lead:]), reversed(t.stride()[lead:])):
+        if n != 1 and s != need:
+            t = t.contiguous()
+            break
+        need *= n
+    stride = t.stride()
+    row = stride[lead - 1] if shape[lead - 1] > 1 else 0
+    return t, (stride[0] if shape[0] > 1 else 0) if lead == 2 else 0, row
 
 
 def _aligned(t, batch, row, lead, d):
@@ -102,11 +107,13 @@ def _forward(x, log_decay, state, cu_seqlens, reverse, out, out_state):
     device, channels = x.device, heads * d
     if out is None:
         y = torch.empty(x.shape, dtype=x.dtype, device=device)
+        y_batch, y_row = _dense((seqs, rows) if lead == 2 else (rows,), lead, channels)
     else:
         y = out
         if out.shape != x.shape or out.dtype != x.dtype or out.get_device() != index:
             raise ValueError("out must match x in shape, dtype and device")
-        if _rows(out, lead, channels)[0] is not out:
+        whole, y_batch, y_row = _rows(out, lead, channels)
+        if whole is not out:
             raise ValueError("out's channels must be contiguous")
     if out_state is None:
         out_state = torch.empty(shape, dtype=torch.float32, device=device)
@@ -122,7 +129,6 @@ def _forward(x, log_decay, state, cu_seqlens, reverse, out, out_state):
     if shared:
         x, x_batch, x_row = _aligned(x, x_batch, x_row, lead, d)
     log_decay, g_batch, g_row = _rows(log_decay, lead, heads if shared else channels)
-    _, y_batch, y_row = _rows(y, lead, channels)
     if state is not None and not state.is_contiguous():
         state = state.contiguous()
     _lib.call_on(index, "vdn_gated_scan", x.data_ptr(), code, x_batch, x_row, log_decay.data_ptr(), g_code, g_batch,
@@ -179,9 +185,6 @@ def gated_scan_backward(grad_y, log_decay, y, *, state=None, grad_state=None, cu
     grad_state is the gradient of the last state, if any; the gradient of the first state
     comes back as fp32 also when `state` was None.  Rows outside the packed sequences
     have zero gradients.  Records nothing for autograd."""
-    if torch.is_grad_enabled():
-        with torch.no_grad():
-            return _backward(grad_y, log_decay, y, state, grad_state, cu_seqlens, bool(reverse))
     return _backward(grad_y, log_decay, y, state, grad_state, cu_seqlens, bool(reverse))
 
 
@@ -205,8 +208,9 @@ def _backward(grad_y, log_decay, y, state, grad_state, cu_seqlens, reverse):
     if shared:
         grad_y, dy_batch, dy_row = _aligned(grad_y, dy_batch, dy_row, lead, d)
         y, y_batch, y_row = _aligned(y, y_batch, y_row, lead, d)
-    _, dx_batch, dx_row = _rows(dx, lead, channels)
-    _, dg_batch, dg_row = _rows(dg, lead, decays)
+    lead_shape = (seqs, rows) if lead == 2 else (rows,)
+    dx_batch, dx_row = _dense(lead_shape, lead, channels)
+    dg_batch, dg_row = _dense(lead_shape, lead, decays)
     if state is not None and not state.is_contiguous():
         state = state.contiguous()
     _lib.call_on(index, "vdn_gated_scan_backward", grad_y.data_ptr(), code, dy_batch, dy_row, log_decay.data_ptr(),
