@@ -91,6 +91,9 @@ def _run(cuda, x, g, cu, reverse, with_state, gen, back=True):
     torch.cuda.synchronize()
     assert y.dtype == dtype and last.dtype == torch.float32
     shared = g.dim() < x.dim()
+    # Below a type's normal range its step is smallest_normal * eps, so a result that lies there
+    # rounds by up to half of that (fp16: 2^-14 * 2^-10 / 2 = 2^-25), however small it is.
+    tiny = lambda t: float(torch.finfo(t).smallest_normal) * torch.finfo(t).eps / 2
     for s in range(seqs):
         rows = slice(cu[s], cu[s + 1]) if packed else slice(None)
         pick = (lambda t: t[rows]) if packed else (lambda t: t[s])
@@ -102,13 +105,13 @@ def _run(cuda, x, g, cu, reverse, with_state, gen, back=True):
         h0 = state[s].double().flatten() if with_state else zero
         ref = _reference(flat(x), gs.flatten(1), h0, flat(dy) if back else None,
                          dlast[s].double().flatten() if with_state else zero, flat(y) if back else None)
-        _close(flat(y), ref["y"], ref["y_err"] + _half(dtype) * (ref["y"].abs() + ref["y_err"]), "y")
+        _close(flat(y), ref["y"], ref["y_err"] + _half(dtype) * (ref["y"].abs() + ref["y_err"]) + tiny(dtype), "y")
         _close(last[s].flatten(), ref["last"], ref["last_err"] + U * ref["last"].abs(), "last")
         if not back:
             continue
         dx, dg, ds = got_back
         assert dx.dtype == dtype and dg.dtype == gd and ds.dtype == torch.float32
-        _close(flat(dx), ref["dx"], ref["dx_err"] + _half(dtype) * (ref["dx"].abs() + ref["dx_err"]), "dx")
+        _close(flat(dx), ref["dx"], ref["dx_err"] + _half(dtype) * (ref["dx"].abs() + ref["dx_err"]) + tiny(dtype), "dx")
         _close(ds[s].flatten(), ref["ds"], ref["ds_err"] + U * ref["ds"].abs(), "ds")
         want, err = ref["dg"], ref["dg_err"]
         if shared:                                        # a sum of d terms, in a tree of at most 9 levels
@@ -118,9 +121,7 @@ def _run(cuda, x, g, cu, reverse, with_state, gen, back=True):
             gotg = turn(pick(dg)).double().cpu()
         else:
             gotg = flat(dg)
-        # below the type's normal range a result rounds by half of its smallest step
-        tiny = float(torch.finfo(gd).smallest_normal) * torch.finfo(gd).eps / 2
-        _close(gotg, want, err + _half(gd) * (want.abs() + err) + tiny, "dg")
+        _close(gotg, want, err + _half(gd) * (want.abs() + err) + tiny(gd), "dg")
     return y, got_back
 
 
@@ -165,6 +166,19 @@ def test_long_runs(cuda, dtype, g_dtype, tokens, reverse):
     """Few tiles and long sequences take 32 tokens a warp: whole and ragged last runs, sharp decays."""
     gen, x, g = _case(tokens, (1, tokens), 2, 36, dtype, g_dtype, False, sharp=True)
     _run(cuda, x, g, None, reverse, True, gen)
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("dtype,g_dtype", [TYPES[0], TYPES[3], TYPES[4]])
+@pytest.mark.parametrize("tokens,reverse", [(1024, True), (1057, False)])
+def test_long_runs_of_shared_decays(cuda, d, dtype, g_dtype, tokens, reverse):
+    gen, x, g = _case(tokens + d, (1, tokens), 2, d, dtype, g_dtype, True, sharp=True)
+    _run(cuda, x, g, None, reverse, True, gen)
+
+
+def test_long_runs_of_shared_decays_packed(cuda):
+    gen, x, g = _case(32, (4200,), 1, 128, torch.bfloat16, torch.float32, True)
+    _run(cuda, x, g, [0, 1, 1100, 1100, 4100], False, True, gen)
 
 
 def test_long_runs_packed_and_strided(cuda):

@@ -174,14 +174,15 @@ constexpr int tile_bytes() {   // of one warp and stage: x (dy), the saved y, th
 // each of which costs a warp some 250 instructions beside its tokens'; runs of 16 leave room
 // for more warps.  The same whatever the alignment, so that strides do not change the order of
 // the sums.
-constexpr int kRun = 16, kLongRun = 32;
+constexpr int kRun = 16, kLongRun = 32;      // half of that where a lane has four channels
+template <int VEC, int L> constexpr bool long_run() { return L * (VEC == 4 ? 2 : 1) >= kLongRun; }
 
 // Warps a CTA, at most.  Runs of 16: the backward per channel keeps the most tiles, so that
 // eight warps would leave one CTA an SM (480 us against 327 on a 1 x 32760 x 5120 backward).
 // Runs of 32: as many as fit the shared memory beside the kernel's fixed arrays.
 template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED>
 constexpr int max_warps() {
-  if (L < kLongRun) return BWD && !SHARED ? 4 : 8;
+  if (!long_run<VEC, L>()) return BWD && !SHARED ? 4 : 8;
   constexpr int line = Lanes<VEC>::N * 32 * (int)sizeof(Fold<typename Lanes<VEC>::V>);
   int w = 8;   // folds of two rounds, of the cluster's CTAs, and sums
   while (w > 1 && w * kStages * tile_bytes<T, TG, VEC, L, BWD, SHARED>() + (3 * w + 2 * MAX_CLUSTER) * line + 1024 > 227 * 1024)
@@ -206,7 +207,7 @@ __device__ __forceinline__ int longest_first(const Params& p, int turn, int lane
 }
 
 template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED, int FROM>
-__global__ void __launch_bounds__(max_warps<T, TG, VEC, L, BWD, SHARED>() * 32, L == kLongRun ? 1 : BWD && !SHARED ? 3 : 2)
+__global__ void __launch_bounds__(max_warps<T, TG, VEC, L, BWD, SHARED>() * 32, long_run<VEC, L>() ? 1 : BWD && !SHARED ? 3 : 2)
     scan_kernel(const Params p, const int cluster, const __grid_constant__ Maps maps) {
   constexpr int GV = SHARED ? 1 : VEC;               // decays per lane and token
   constexpr int TILE = 32 * VEC, MAX_WARPS = max_warps<T, TG, VEC, L, BWD, SHARED>();
@@ -715,7 +716,7 @@ static int choose_shape(int64_t mean, int64_t longest, int64_t seqs, bool sorted
   const int64_t ids = seqs * tiles;
   int64_t best = -1;
   const int most = warps;
-  for (int w = most; w == most || w >= (L == kLongRun ? 2 : 4); w /= 2) {
+  for (int w = most; w == most || w >= (long_run<VEC, L>() ? 2 : 4); w /= 2) {
     const int64_t runs = (mean + w * L - 1) / (w * L), most_runs = (longest + w * L - 1) / (w * L);
     for (int c = 1; c <= MAX_CLUSTER && c <= (most_runs > 1 ? most_runs : 1); ++c) {
       int& fit = places[dev][w == 8 ? 3 : w >> 1][c];   // clusters resident at once
@@ -730,7 +731,7 @@ static int choose_shape(int64_t mean, int64_t longest, int64_t seqs, bool sorted
       const int64_t waves = (ids + fit - 1) / fit, tail = ids - (waves - 1) * fit;
       auto load = [&](int64_t clusters) {
         const int64_t on_sm = w * ((clusters * c + 147) / 148);
-        if (L < kLongRun) return (SHARED ? 8 : 4) + on_sm;
+        if (!long_run<VEC, L>()) return (SHARED ? 8 : 4) + on_sm;
         const int64_t t = 2 + (on_sm + 3) / 4 * 4;
         return t > 6 ? t : 6;
       };
@@ -842,8 +843,14 @@ static int dispatch(Params& p, int shared_dim, cudaStream_t stream) {
     const int vec = shared_dim / 32;
     VDN_CHECK_ARG(fits(vec), "a shared decay needs rows aligned to %d elements", vec);
     p.tiles = (int)(p.channels / shared_dim);
+    // Long runs as below, us without and with: 4 tiles of 16384 x 128 81 and 48 (backward 95 and 58),
+    // 16 tiles 97 and 87 (117 and 101), 80 tiles of 16384 x 64 123 and 155 (153 and 183).
+    const bool few = p.seqs * p.tiles <= 37 && mean_length(p) >= 1024;
+    if (vec == 4 && few) return launch<T, TG, 4, kLongRun / 2, BWD, true>(p, stream);
     if (vec == 4) return launch<T, TG, 4, kRun / 2, BWD, true>(p, stream);
+    if (vec == 2 && few) return launch<T, TG, 2, kLongRun, BWD, true>(p, stream);
     if (vec == 2) return launch<T, TG, 2, kRun, BWD, true>(p, stream);
+    if (few) return launch<T, TG, 1, kLongRun, BWD, true>(p, stream);
     return launch<T, TG, 1, kRun, BWD, true>(p, stream);
   }
   const int vec = fits(2) ? 2 : 1;
