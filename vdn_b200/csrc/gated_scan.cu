@@ -33,7 +33,8 @@
 // factor: hi = fp32(1 + e), lo = e - (hi - 1), e = expm1(r) with r = g - n ln 2 in [-0.35,
 // 0.35] from a polynomial fitted at Chebyshev nodes (2.5e-8 relative).  It runs on packed
 // fp32 pairs with no branch and no MUFU operation.  A run's A comes from the sum of its g, not
-// from the product of its rounded decays.  exp(g) is 0 below g = -87.7.
+// from the product of its rounded decays; the sum takes g before it is clamped, so that a -inf stays one
+// however much growth stands beside it.  exp(g) is 0 below g = -87.7 and inf above 88.37.
 #include <initializer_list>
 #include <type_traits>
 
@@ -100,20 +101,18 @@ template <> __device__ __forceinline__ uint32_t clamp_word<__half>(uint32_t w) {
   asm("{\n\t.reg .b32 t;\n\tmax.NaN.f16x2 t, %1, %2;\n\tmin.NaN.f16x2 %0, t, %3;\n\t}" : "=r"(r) : "r"(w), "r"(0xD57ED57Eu), "r"(0x55885588u));
   return r;
 }
+// The log decays as they are, for a run's sum (a -inf must stay one beside growth), and held.
 template <typename TG, int GV, typename V, int N>
-__device__ __forceinline__ void unpack_decays(const Raw<TG, GV>& raw, V (&g)[N]) {
+__device__ __forceinline__ void unpack_decays(const Raw<TG, GV>& raw, V (&g)[N], V (&held)[N]) {
+  unpack_lanes<TG, GV>(raw, g);
   if constexpr (GV * sizeof(TG) < 4) {
-    float e[1];
-    unpack<TG, 1>(raw, e);
-    e[0] = clamp_decay(e[0]);
-    to_lanes(e, g);
+    held[0] = clamp_decay(g[0]);
   } else {
     uint32_t w[GV * sizeof(TG) / 4];
     words(raw, w);
 #pragma unroll
     for (auto& x : w) x = clamp_word<TG>(x);
-    const auto held = join(w);
-    unpack_lanes<TG, GV>(held, g);
+    unpack_lanes<TG, GV>(join(w), held);
   }
 }
 
@@ -328,7 +327,7 @@ __global__ void __launch_bounds__(max_warps<T, TG, VEC, L, BWD, SHARED>() * 32, 
     const bool in = lane < L && i + lane < len;
     float e[1] = {0.f};
     if (in) unpack<TG, 1>(*reinterpret_cast<const Raw<TG, 1>*>(pg + (i + lane) * sg), e);
-    return clamp_decay(e[0]);
+    return e[0];
   };
   float g_next = SHARED ? load_shared(i0) : 0.f;
 
@@ -373,7 +372,7 @@ __global__ void __launch_bounds__(max_warps<T, TG, VEC, L, BWD, SHARED>() * 32, 
     }
     float hi_lane = 1.f, lo_lane = 0.f;
     if constexpr (SHARED) {
-      decay_pair(g_next, hi_lane, lo_lane);
+      decay_pair(clamp_decay(g_next), hi_lane, lo_lane);
       float s = g_next;
 #pragma unroll
       for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -384,18 +383,18 @@ __global__ void __launch_bounds__(max_warps<T, TG, VEC, L, BWD, SHARED>() * 32, 
 #pragma unroll
       for (int l = 0; l < L; ++l) {
         V x[NV];
-        G g[NG], hi[NG], lo[NG];
+        G g[NG], held[NG], hi[NG], lo[NG];
         unpack_lanes<T, VEC>(RING ? *x_at(l) : rx[RING ? 0 : l], x);
         if constexpr (SHARED) {
           hi[0] = vset(G{}, __shfl_sync(0xffffffffu, hi_lane, l));
           lo[0] = vset(G{}, __shfl_sync(0xffffffffu, lo_lane, l));
         } else {
-          unpack_decays<TG, GV>(RING ? *g_at(l) : rg[RING || SHARED ? 0 : l], g);
+          unpack_decays<TG, GV>(RING ? *g_at(l) : rg[RING || SHARED ? 0 : l], g, held);
         }
 #pragma unroll
         for (int v = 0; v < NG; ++v) {
           if constexpr (!SHARED) {
-            decay_pair(g[v], hi[v], lo[v]);
+            decay_pair(held[v], hi[v], lo[v]);
             sum[v] = vadd(sum[v], g[v]);
           }
           far[v] = vmul(far[v], hi[v]);
