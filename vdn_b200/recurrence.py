@@ -105,6 +105,7 @@ def _aligned(t, batch, row, lead, d):
 def _forward(x, log_decay, state, cu_seqlens, reverse, out, out_state):
     index, code, g_code, lead, seqs, rows, heads, d, shared, shape = _layout(x, log_decay, state, cu_seqlens, "x")
     device, channels = x.device, heads * d
+    given = [t for t in (out, out_state) if t is not None]
     if out is None:
         y = torch.empty(x.shape, dtype=x.dtype, device=device)
         y_batch, y_row = _dense((seqs, rows) if lead == 2 else (rows,), lead, channels)
@@ -135,6 +136,8 @@ def _forward(x, log_decay, state, cu_seqlens, reverse, out, out_state):
                  g_row, shared, None if state is None else state.data_ptr(),
                  None if cu_seqlens is None else cu_seqlens.data_ptr(), seqs, rows, heads, d, reverse, y.data_ptr(),
                  y_batch, y_row, out is None, out_state.data_ptr(), status_address(device))
+    if given:                                        # written past autograd's sight: graphs that saved them must fail
+        torch.autograd.graph.increment_version(given)
     return y, out_state
 
 
@@ -171,7 +174,7 @@ def gated_scan(x, log_decay, state=None, *, cu_seqlens=None, reverse=False, out=
     its last row to its first.  Strided rows and expanded log_decay are read in place as
     long as a row's channels are contiguous.  A state that overflows fp32 comes out as inf or NaN.
     """
-    if torch.is_grad_enabled() and _lib.records(x, log_decay, state):
+    if torch.is_grad_enabled() and _lib.records(x, log_decay, state, out, out_state):
         if out is not None or out_state is not None:
             raise ValueError("out and out_state cannot be given where gradients are recorded")
         _lib.refuse_captured_autograd("gated_scan", x)
