@@ -400,7 +400,8 @@ int vdn_vda_forward_noalloc(const void* q, const void* k, const void* v, int64_t
  * empty sequences allowed).  reverse: each sequence runs from its last row to its first.
  * dtype: x and y; g_dtype: log_decay, the same or fp32.  shared: one decay per head
  * ([.., heads], d 32, 64 or 128).  state / out_state: fp32 [seqs, heads * d] or NULL (zeros
- * in / not wanted); out_state may be state.  zero_tail: write zeros to the rows in
+ * in / not wanted); out_state may be state and y may be x or log_decay, strides included, but outputs share
+ * no other memory with inputs or each other.  zero_tail: write zeros to the rows in
  * front of the first packed sequence and behind the last, else they are left alone.  rows and channels below 2^30, row strides
  * below 2^26.  States and sums are fp32 and added in a fixed order.  status: as in vdn_mxfp8_gemm.
  * Per-token companion of the frame-wise scan, src/models/linear_attention/scan.py:270-355. */

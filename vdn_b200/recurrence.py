@@ -102,10 +102,66 @@ def _aligned(t, batch, row, lead, d):
     return t, batch, row
 
 
+def _span(t):
+    """(first address, the one behind the last) of t's values."""
+    start = t.data_ptr()
+    if t.is_contiguous():
+        return start, start + t.nbytes
+    return start, start + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+
+
+def _meets(a, b):
+    """Whether the address ranges of a and b meet."""
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1 and a.numel() > 0 and b.numel() > 0
+
+
+def _same(a, b):
+    return a.data_ptr() == b.data_ptr() and a.dtype == b.dtype and a.shape == b.shape and a.stride() == b.stride()
+
+
+def _beside(a, b, lead):
+    """Whether a's and b's rows are different columns of rows of one buffer: no address in both."""
+    steps = [(p, q) for n, p, q in zip(a.shape[:lead], a.stride(), b.stride()) if n > 1]
+    if not steps or a.element_size() != b.element_size() or a.shape[:lead] != b.shape[:lead]:
+        return False
+    pitch = min(p for p, _ in steps)
+    wide, narrow = a.shape[lead:].numel(), b.shape[lead:].numel()
+    if pitch < 1 or any(p != q or p % pitch for p, q in steps):
+        return False
+    off = (b.data_ptr() - a.data_ptr()) // a.element_size() % pitch
+    return off >= wide and off + narrow <= pitch
+
+
+def _check_memory(x, log_decay, state, out, out_state, lead):
+    """Refuses outputs whose memory a row or state still to be read, or another output, shares: the
+    order in which rows are read and written is not that of the recurrence."""
+    step = lead == 2 and x.shape[1] == 1              # each value is read and written by one thread
+    if out is not None:
+        for n, s in zip(out.shape[:lead], out.stride()):
+            if n > 1 and s < out.shape[lead:].numel():
+                raise ValueError("out's rows must not overlap")
+        for t, name in ((x, "x"), (log_decay, "log_decay")):
+            if _meets(out, t) and not _same(out, t) and not _beside(out, t, lead):
+                raise ValueError(f"out and {name} must be the same rows or share no memory")
+        for t, name in ((state, "state"), (out_state, "out_state")):
+            if t is not None and _meets(out, t) and not (step and out.data_ptr() == t.data_ptr() and
+                                                         out.dtype == t.dtype and out.is_contiguous()):
+                raise ValueError(f"out and {name} must not share memory")
+    if out_state is not None:
+        if state is not None and out_state is not state and _meets(out_state, state) and not _same(out_state, state):
+            raise ValueError("out_state and state must be the same memory or share none")
+        for t, name in ((x, "x"), (log_decay, "log_decay")):
+            if _meets(out_state, t) and not (step and out_state.data_ptr() == t.data_ptr() and t.dtype == torch.float32 and
+                                             t.numel() == out_state.numel() and t.is_contiguous()):
+                raise ValueError(f"out_state and {name} must not share memory")
+
+
 def _forward(x, log_decay, state, cu_seqlens, reverse, out, out_state):
     index, code, g_code, lead, seqs, rows, heads, d, shared, shape = _layout(x, log_decay, state, cu_seqlens, "x")
     device, channels = x.device, heads * d
     given = [t for t in (out, out_state) if t is not None]
+    own_state = out_state
     if out is None:
         y = torch.empty(x.shape, dtype=x.dtype, device=device)
         y_batch, y_row = _dense((seqs, rows) if lead == 2 else (rows,), lead, channels)
@@ -132,6 +188,8 @@ def _forward(x, log_decay, state, cu_seqlens, reverse, out, out_state):
     log_decay, g_batch, g_row = _rows(log_decay, lead, heads if shared else channels)
     if state is not None and not state.is_contiguous():
         state = state.contiguous()
+    if given:
+        _check_memory(x, log_decay, state, out, own_state, lead)
     _lib.call_on(index, "vdn_gated_scan", x.data_ptr(), code, x_batch, x_row, log_decay.data_ptr(), g_code, g_batch,
                  g_row, shared, None if state is None else state.data_ptr(),
                  None if cu_seqlens is None else cu_seqlens.data_ptr(), seqs, rows, heads, d, reverse, y.data_ptr(),
@@ -170,7 +228,8 @@ def gated_scan(x, log_decay, state=None, *, cu_seqlens=None, reverse=False, out=
     channel.  With cu_seqlens (int32 [S + 1] on the device, nondecreasing row offsets) the
     sequences lie end to end: x [N, C] or [N, H, d]; rows in front of the first offset and
     behind the last come back zero, and stay as they were in a caller's `out`.  state / out_state fp32 [B or S, C] or
-    [.., H, d]; out_state may be `state` (updated in place).  reverse runs each sequence from
+    [.., H, d]; out_state may be `state` and out may be x or log_decay (updated in place); other shared
+    memory is refused.  reverse runs each sequence from
     its last row to its first.  Strided rows and expanded log_decay are read in place as
     long as a row's channels are contiguous.  A state that overflows fp32 comes out as inf or NaN.
     """
