@@ -13,6 +13,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "libvdn_b200.so"
 
@@ -154,6 +155,15 @@ def records(*tensors) -> bool:
         if t is not None and t.requires_grad:
             return True
     return False
+
+
+def refuse_tangents(name: str, *tensors) -> None:
+    """Forward-mode derivatives are not implemented: a call on a dual tensor must not drop its tangent."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name} has no forward-mode derivative (an argument carries a tangent)")
 
 
 def capturing(device: torch.device) -> bool:

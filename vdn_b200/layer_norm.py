@@ -68,6 +68,7 @@ def _like(t):
 
 
 def _forward(x, weight, bias, eps, stats):
+    _lib.refuse_tangents("layer_norm", x, weight, bias)
     index, width, code, w_code = _check(x, weight, bias)
     flat, rows, ld = _rows(x, width)
     y = _like(x)
@@ -114,6 +115,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, return_stats=False):
 
 
 def _backward(grad_y, x, weight, mean, rstd, want_w, want_b, bias_dtype=None):
+    _lib.refuse_tangents("layer_norm_backward", grad_y, x, weight, mean, rstd)
     index, width, code, kind = _check(x, weight, None)
     if grad_y.shape != x.shape or grad_y.dtype != x.dtype or grad_y.get_device() != index:
         raise ValueError("grad_y must match x in shape, dtype and device")

@@ -62,6 +62,7 @@ def _same(t, x, index, shape, name):
 
 
 def _forward(x, weight, bias, act, residual, want_pre):
+    _lib.refuse_tangents("linear_act", x, weight, bias, residual)
     index, code = _check(x, weight, act)
     n, k = weight.shape
     shape = (*x.shape[:-1], n)
@@ -125,6 +126,7 @@ def linear_act(x, weight, bias=None, *, act="none", residual=None, return_pre=Fa
 
 
 def _backward(grad_y, x, weight, pre, act, want_x, want_w, want_b):
+    _lib.refuse_tangents("linear_act_backward", grad_y, x, weight, pre)
     index, dtype = _check(x, weight, act)
     n, k = weight.shape
     shape = (*x.shape[:-1], n)

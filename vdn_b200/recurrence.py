@@ -158,6 +158,7 @@ def _check_memory(x, log_decay, state, out, out_state, lead):
 
 
 def _forward(x, log_decay, state, cu_seqlens, reverse, out, out_state):
+    _lib.refuse_tangents("gated_scan", x, log_decay, state, out, out_state)
     index, code, g_code, lead, seqs, rows, heads, d, shared, shape = _layout(x, log_decay, state, cu_seqlens, "x")
     device, channels = x.device, heads * d
     given = [t for t in (out, out_state) if t is not None]
@@ -251,6 +252,7 @@ def gated_scan_backward(grad_y, log_decay, y, *, state=None, grad_state=None, cu
 
 
 def _backward(grad_y, log_decay, y, state, grad_state, cu_seqlens, reverse):
+    _lib.refuse_tangents("gated_scan_backward", grad_y, log_decay, y, state, grad_state)
     index, code, g_code, lead, seqs, rows, heads, d, shared, shape = _layout(y, log_decay, state, cu_seqlens, "y")
     if grad_y.shape != y.shape or grad_y.dtype != y.dtype or grad_y.get_device() != index:
         raise ValueError("grad_y must match y in shape, dtype and device")
