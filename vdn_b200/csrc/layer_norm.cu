@@ -15,8 +15,8 @@
 // them; one line of partial sums per CTA goes to the caller's workspace, and a second
 // kernel adds the lines in a fixed order.  No atomics: the same bits on every run.
 // Widths that fit no register form take `wide` kernels, which read a row again for each pass.
-// Bound by HBM: 32760 x 5120 in bf16 forward 124 us (5.4 TB/s, a copy reaches 6.5), backward 199
-// (5.1 TB/s, some 10 us of it the sum of the lines).
+// Bound by HBM: 32760 x 5120 in bf16 forward 124 us (5.4 TB/s, a copy reaches 6.5), backward 204
+// (4.9 TB/s, some 10 us of it the sum of the lines).
 #include <initializer_list>
 
 #include "train_common.cuh"
@@ -621,9 +621,10 @@ __global__ void __launch_bounds__(MAXT, PER_SM) backward_ring_kernel(const Bwd p
     for (int r = 0; r < ROWS; ++r) {
       const float s1 = __shfl_sync(0xffffffffu, s, 2 * r * SHARE), s2 = __shfl_sync(0xffffffffu, s, (2 * r + 1) * SHARE);
       if (r >= n) continue;
-      // dx = q t - q s1 - q xh s2 with xh = (x - m) q: one scale and one offset per row
-      const float slope = -s2 * inv * q[r] * q[r];
-      const V scale = vset(V{}, q[r]), c2 = vset(V{}, slope), c1 = vset(V{}, fmaf(-m[r], slope, -s1 * inv * q[r]));
+      // dx = q t - q s1 - q xh s2 with xh = (x - m) q.  x is centred first: the mean folded into the
+      // offset saves an addition a value but leaves x slope and m slope to cancel, an error of u |m| / std
+      const V minus = vset(V{}, -m[r]), scale = vset(V{}, q[r]), c2 = vset(V{}, -s2 * inv * q[r] * q[r]),
+              c1 = vset(V{}, -s1 * inv * q[r]);
       T* dx = static_cast<T*>(p.dx) + (row + r) * p.dx_ld;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
@@ -635,7 +636,7 @@ __global__ void __launch_bounds__(MAXT, PER_SM) backward_ring_kernel(const Bwd p
         weights(k, col, w);
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-          x[i] = vfma(x[i], c2, vfma(vmul(w[i], d[i]), scale, c1));
+          x[i] = vfma(vadd(x[i], minus), c2, vfma(vmul(w[i], d[i]), scale, c1));
         }
         store_once(dx + col, pack_lanes<T, VEC>(x));
       }
