@@ -83,7 +83,9 @@ __device__ __forceinline__ f2 act_slope2(f2 z) {
   float v0, v1, a, b, q0, q1, p0, p1;
   f2_unpack(v, v0, v1);
   f2_unpack(f2_mul(f2_pack(fabsf(v0), fabsf(v1)), c2(-1.4426950408889634f)), a, b);
-  const f2 e = f2_pack(ex2_approx(a), ex2_approx(b));
+  // fmaxf: a NaN's exponential becomes 0, so that the shared reciprocal stays its neighbour's; its own
+  // slope is NaN through cdv
+  const f2 e = f2_pack(ex2_approx(fmaxf(a, -150.f)), ex2_approx(fmaxf(b, -150.f)));
   f2_unpack(f2_add(e, c2(1.0f)), a, b);
   const float q = rcp_approx(a * b);
   const f2 r = f2_mul(f2_pack(b, a), c2(q)), er = f2_mul(e, r);
