@@ -43,7 +43,7 @@ enum { NONE = VDN_ACT_NONE, TANH = VDN_ACT_GELU_TANH, ERF = VDN_ACT_GELU_ERF, SI
 template <int ACT>
 __device__ __forceinline__ float act_value(float z) {
   if constexpr (ACT == NONE) return z;
-  if constexpr (ACT == ERF) return 0.5f * z * (1.0f + erff(z * 0.7071067811865476f));
+  if constexpr (ACT == ERF) return 0.5f * z * erfcf(z * -0.7071067811865476f);   // 1 + erf cancels below z = -3
   const float v = ACT == TANH ? 1.5957691216057308f * fmaf(0.044715f * z * z, z, z) : z;
   return __fdividef(z, 1.0f + __expf(-v));   // exp overflow: z / inf = 0
 }
@@ -54,7 +54,7 @@ __device__ __forceinline__ float act_slope(float z) {
   float c;                                   // past 30 the slope is 0 or 1; NaN stays NaN
   asm("max.NaN.f32 %0, %1, 0fC1F00000;\n\tmin.NaN.f32 %0, %0, 0f41F00000;" : "=f"(c) : "f"(z));
   if constexpr (ACT == ERF)
-    return 0.5f * (1.0f + erff(c * 0.7071067811865476f)) + c * 0.3989422804014327f * __expf(-0.5f * c * c);
+    return 0.5f * erfcf(c * -0.7071067811865476f) + c * 0.3989422804014327f * __expf(-0.5f * c * c);
   const float k = 1.5957691216057308f;
   const float v = ACT == TANH ? k * fmaf(0.044715f * c * c, c, c) : c;
   const float dv = ACT == TANH ? k * fmaf(0.134145f * c, c, 1.0f) : 1.0f;
