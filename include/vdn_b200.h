@@ -51,6 +51,10 @@ const char* vdn_last_error(void);
 int vdn_abi_version(void);
 /* *supported = 1 when `device` is an sm_100 part this library was built for. */
 int vdn_device_supported(int device, int* supported);
+/* A status word of `device` for the entry points below that take `status`: pinned host memory that the
+ * device writes, so the host reads it (and sets it back to 0) without a copy.  It lives as long as the process,
+ * may be fetched during a stream capture, and is the same for every call with that device. */
+int vdn_status_word(int device, int** word);
 
 /* ------------------------------------------------------------------ MXFP8 */
 

@@ -10,5 +10,6 @@ and, per token and with gradients, the operators of a recurrent mixing layer:
 All compute runs in libvdn_b200.so (include/vdn_b200.h); there is no fallback.
 """
 from . import _lib  # noqa: F401
+from ._lib import check_status
 
-__all__ = ["_lib"]
+__all__ = ["_lib", "check_status"]

@@ -29,6 +29,7 @@ SIGNATURES = {
     "vdn_last_error": (C.c_char_p, []),
     "vdn_abi_version": (_i32, []),
     "vdn_device_supported": (_i32, [_i32, C.POINTER(_i32)]),
+    "vdn_status_word": (_i32, [_i32, C.POINTER(_p)]),
     "vdn_mxfp8_padded_shape": (_i32, [_i64, _i64, C.POINTER(_i64), C.POINTER(_i64)]),
     "vdn_mxfp8_quantize": (_i32, [_p, _i64, _i64, _i64, _p, _p, _p, _p]),
     "vdn_mxfp8_act_quantize": (_i32, [_i32, _p, _i64, _i64, _i64, _p, _p, _p, _p]),
@@ -139,6 +140,36 @@ def call_on(index: int, name: str, *args) -> None:
             rc = fn(*args, _raw_stream(index))
     if rc != VDN_OK:
         raise_status(rc)
+
+
+# Per device the word that the per-token operators' kernels set when a wait inside them gave up.
+_WORDS: dict[int, C.c_int32] = {}
+
+
+def status_word(index: int) -> int:
+    """The address of device `index`'s status word.  Raises if an earlier call's kernel has set it:
+    kernels run behind their calls, so a wait that gave up is reported by the next call (or by
+    check_status)."""
+    word = _WORDS.get(index)
+    if word is None:
+        at = _p()
+        with torch.cuda.device(index):
+            call("vdn_status_word", index, C.byref(at))
+        word = _WORDS[index] = C.c_int32.from_address(at.value)
+    if word.value:
+        word.value = 0
+        raise RuntimeError(f"a wait inside an earlier gated_scan, layer_norm or linear_act kernel on cuda:{index} gave up; "
+                           "results since then are not valid")
+    return C.addressof(word)
+
+
+def check_status(device=None) -> None:
+    """Waits for `device` (the current one by default) and raises RuntimeError if a wait inside one of the
+    per-token operators' kernels gave up since the last report."""
+    device = torch.device("cuda" if device is None else device)
+    index = torch.cuda.current_device() if device.index is None else device.index
+    torch.cuda.synchronize(index)
+    status_word(index)
 
 
 def device_index(t: torch.Tensor, what: str) -> int:

@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .mxfp8_linear import _status
+from .mxfp8_linear import status_address
 
 __all__ = ["gate_gemm"]
 
@@ -51,7 +51,7 @@ def gate_gemm(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None
         # rows padded to a multiple of 8 elements (the store map's 16-byte row pitch)
         target = torch.empty(rows, (n + 7) // 8 * 8, device=x.device, dtype=torch.bfloat16)[:, :n]
     _lib.call("vdn_gate_gemm", _lib.ptr(x), x.stride(0), _lib.ptr(w), w.stride(0), _lib.ptr(bias), rows, n, k,
-              n_sig, _lib.ptr(target), target.stride(0), _lib.ptr(_status(x.device)), _lib.stream_of(x.device))
+              n_sig, _lib.ptr(target), target.stride(0), status_address(x.device), _lib.stream_of(x.device))
     if out is not None and target is not out:
         out.copy_(target)
         return out

@@ -17,7 +17,6 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .mxfp8_linear import status_address
 
 __all__ = ["layer_norm", "layer_norm_backward"]
 
@@ -136,7 +135,7 @@ def _backward(grad_y, x, weight, mean, rstd, want_w, want_b, bias_dtype=None):
     _lib.call_on(index, "vdn_layer_norm_backward", dy.data_ptr(), code, rows, width, dy_ld, flat.data_ptr(), x_ld,
                  None if w is None else w.data_ptr(), kind, mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), width,
                  dw.data_ptr() if want_w else None, db.data_ptr() if want_b else None, ws.data_ptr(), need,
-                 status_address(device))
+                 _lib.status_word(index))
     return dx, dw, db
 
 

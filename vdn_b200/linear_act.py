@@ -16,7 +16,6 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .mxfp8_linear import status_address
 
 __all__ = ["linear_act", "linear_act_backward", "ACTIVATIONS"]
 
@@ -87,7 +86,7 @@ def _forward(x, weight, bias, act, residual, want_pre):
     _lib.call_on(index, "vdn_linear_act", px, ldx, pw, ldw, None if bias is None else bias.data_ptr(),
                  None if res is None else res.data_ptr(), ldr, code, ACTIVATIONS[act], rows, n, k, y.data_ptr(), n,
                  None if pre is None else pre.data_ptr(), n, None if ws is None else ws.data_ptr(), need,
-                 status_address(device))
+                 _lib.status_word(index))
     return y, pre
 
 
@@ -149,7 +148,7 @@ def _backward(grad_y, x, weight, pre, act, want_x, want_w, want_b):
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     _lib.call_on(index, "vdn_linear_act_backward", pdy, ldy, None if z is None else z.data_ptr(), ldp, px, ldx, pw, ldw,
                  dtype, code, rows, n, k, dx.data_ptr() if want_x else None, k, dw.data_ptr() if want_w else None, k,
-                 db.data_ptr() if want_b else None, ws.data_ptr(), need, status_address(dev))
+                 db.data_ptr() if want_b else None, ws.data_ptr(), need, _lib.status_word(index))
     return dx, dw, db
 
 

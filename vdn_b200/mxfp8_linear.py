@@ -82,7 +82,7 @@ def mxfp8_gemm(data, scales, weight_data, weight_scale, n, *, rows, bias=None, o
     if rows:
         _lib.call("vdn_mxfp8_gemm", _lib.ptr(data), _lib.ptr(scales), _lib.ptr(weight_data),
                   _lib.ptr(weight_scale), _lib.ptr(bias), m_pad, n, n_pad, k_pad, rows, _lib.ptr(y),
-                  y.stride(0), _lib.ptr(_status(data.device)), _lib.stream_of(data.device))
+                  y.stride(0), status_address(data.device), _lib.stream_of(data.device))
     return y
 
 

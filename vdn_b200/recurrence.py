@@ -16,7 +16,6 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .mxfp8_linear import status_address
 
 __all__ = ["gated_scan", "gated_scan_backward"]
 
@@ -194,7 +193,7 @@ def _forward(x, log_decay, state, cu_seqlens, reverse, out, out_state):
     _lib.call_on(index, "vdn_gated_scan", x.data_ptr(), code, x_batch, x_row, log_decay.data_ptr(), g_code, g_batch,
                  g_row, shared, None if state is None else state.data_ptr(),
                  None if cu_seqlens is None else cu_seqlens.data_ptr(), seqs, rows, heads, d, reverse, y.data_ptr(),
-                 y_batch, y_row, out is None, out_state.data_ptr(), status_address(device))
+                 y_batch, y_row, out is None, out_state.data_ptr(), _lib.status_word(index))
     if given:                                        # written past autograd's sight: graphs that saved them must fail
         torch.autograd.graph.increment_version(given)
     return y, out_state
@@ -281,5 +280,5 @@ def _backward(grad_y, log_decay, y, state, grad_state, cu_seqlens, reverse):
                  g_code, g_batch, g_row, shared, y.data_ptr(), y_batch, y_row, None if state is None else state.data_ptr(),
                  None if grad_state is None else grad_state.data_ptr(),
                  None if cu_seqlens is None else cu_seqlens.data_ptr(), seqs, rows, heads, d, reverse, dx.data_ptr(),
-                 dx_batch, dx_row, dg.data_ptr(), dg_batch, dg_row, True, ds.data_ptr(), status_address(device))
+                 dx_batch, dx_row, dg.data_ptr(), dg_batch, dg_row, True, ds.data_ptr(), _lib.status_word(index))
     return dx, dg, ds
