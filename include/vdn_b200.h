@@ -437,7 +437,7 @@ int vdn_layer_norm(const void* x, int dtype, int64_t rows, int64_t width, int64_
 
 /* Gradients of vdn_layer_norm: dx (dtype), d_weight and d_bias (w_dtype, either may be
  * NULL), the two summed over the rows in fp32 and in a fixed order through the workspace.
- * status: as in vdn_mxfp8_gemm. */
+ * The workspace is aligned to fp32 values.  status: as in vdn_mxfp8_gemm. */
 size_t vdn_layer_norm_backward_workspace_size(int64_t rows, int64_t width);
 int vdn_layer_norm_backward(const void* dy, int dtype, int64_t rows, int64_t width, int64_t dy_stride,
                             const void* x, int64_t x_stride, const void* weight, int w_dtype,
@@ -449,7 +449,7 @@ int vdn_layer_norm_backward(const void* dy, int dtype, int64_t rows, int64_t wid
  * accumulation: z = x w^T + bias, pre = z (if not NULL), y = act(z) + residual (if not
  * NULL).  x [rows, k], w [n, k], bias [n], residual, y and pre [rows, n]; columns contiguous,
  * row strides in elements.  x or w whose address or stride is not a multiple of 16 bytes is
- * copied into the workspace first (vdn_linear_workspace_size; 0 and NULL otherwise).  y
+ * copied into the workspace first (vdn_linear_workspace_size, 16-byte aligned; 0 and NULL otherwise).  y
  * must not overlap the inputs.  act: VDN_ACT_NONE, _GELU_TANH, _GELU_ERF or _SILU.  status:
  * as in vdn_mxfp8_gemm.  The 16-bit, trainable counterpart of the block's MXFP8
  * projections with fused epilogues (src/models/ops/mxfp8_linear.py:60-102). */
@@ -463,7 +463,8 @@ int vdn_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const
 /* Gradients of vdn_linear_act from dy and its `pre` (not read for VDN_ACT_NONE): with dz = dy
  * act'(pre), dx = dz w, dw = dz^T x and d_bias = the column sums of dz, each left out when
  * NULL.  dz is rounded to dtype for the two products; d_bias sums it unrounded, in fp32 and a
- * fixed order.  The residual's gradient is dy. */
+ * fixed order.  The residual's gradient is dy.  The workspace is 16-byte aligned.  In fp16 a dz above 65504
+ * becomes infinite (|act'| stays below 1.13, so only where dy is near that limit itself). */
 size_t vdn_linear_backward_workspace_size(const void* dy, int64_t ldy, const void* x, int64_t ldx,
                                           const void* w, int64_t ldw, int act, int64_t rows, int64_t n,
                                           int64_t k);

@@ -916,6 +916,7 @@ extern "C" int vdn_layer_norm_backward(const void* dy, int dtype, int64_t rows, 
   VDN_CHECK_ARG(rows == 1 || (dy_stride >= 0 && x_stride >= 0 && dx_stride >= width), "bad row stride");
   VDN_CHECK_ARG(workspace_bytes >= vdn_layer_norm_backward_workspace_size(rows, width),
                 "workspace smaller than vdn_layer_norm_backward_workspace_size");
+  VDN_CHECK_ARG(aligned_to(workspace, sizeof(float)), "the workspace must be aligned to fp32 values");
   const Bwd p = {dy, x, weight, mean, rstd, dx, static_cast<float*>(workspace), rows, dy_stride, x_stride, dx_stride,
                  (int)width, status};
   VDN_LN_DISPATCH(backward, p, d_weight, d_bias, stream)

@@ -922,6 +922,7 @@ static int settle(std::initializer_list<Matrix> operands, uint8_t*& ws, size_t& 
     const size_t bytes = padded_bytes(o.base, o.ld, o.rows, o.cols);
     if (!bytes) continue;
     VDN_CHECK_ARG(ws && bytes <= left, "workspace smaller than the padded operands need");
+    VDN_CHECK_ARG(aligned16(ws), "the workspace must be 16-byte aligned");
     p.src[n] = static_cast<const uint16_t*>(o.base);
     p.dst[n] = reinterpret_cast<uint16_t*>(ws);
     p.rows[n] = o.rows;
@@ -1058,6 +1059,7 @@ static int backward(const void* dy, int64_t ldy, const void* pre, int64_t ldp, c
   if (db) {
     part = reinterpret_cast<float*>(take(part_bytes(n)));
     VDN_CHECK_ARG(part, "workspace smaller than vdn_linear_backward_workspace_size");
+    VDN_CHECK_ARG(aligned_to(part, sizeof(float)), "the workspace must be 16-byte aligned");
   }
   const void* dz = dy;
   int64_t ldz = ldy;
@@ -1065,6 +1067,7 @@ static int backward(const void* dy, int64_t ldy, const void* pre, int64_t ldp, c
   if (act != NONE) {
     out = take(dz_bytes(dy, ldy, act, rows, n));
     VDN_CHECK_ARG(out, "workspace smaller than vdn_linear_backward_workspace_size");
+    VDN_CHECK_ARG(aligned16(out), "the workspace must be 16-byte aligned");
     dz = out;
     ldz = pad8(n);
   }

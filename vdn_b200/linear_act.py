@@ -155,6 +155,7 @@ def _backward(grad_y, x, weight, pre, act, want_x, want_w, want_b):
 def linear_act_backward(grad_y, x, weight, pre=None, *, act="none", bias=True):
     """(grad of x, of weight, of bias or None) from the forward's inputs and `pre`.  The residual's
     gradient is grad_y.  The activation's gradient enters the two products rounded to the
-    operands' type; the bias gradient sums it unrounded, in fp32 and a fixed order.  Records
+    operands' type (in fp16 it is infinite above 65504, which takes a grad_y near that limit: the
+    slopes stay below 1.13); the bias gradient sums it unrounded, in fp32 and a fixed order.  Records
     nothing for autograd."""
     return _backward(grad_y, x, weight, pre, act, True, True, bool(bias))
