@@ -112,94 +112,61 @@ struct Weights {
   }
 };
 
-// Each CTA walks rows (blockIdx.x, + gridDim.x, ..) with the next row's loads in flight and the
-// weights of its columns in registers (HELD; else read again for every row, from L1).
-template <typename T, typename TW, int VEC, int NV, int LANES, int MAXT, int PER_SM, bool HELD>
-__global__ void __launch_bounds__(MAXT, PER_SM) forward_kernel(const Fwd p) {
+// Short rows, one vector a lane: a group of LANES lanes walks rows (its CTA's blockIdx.x, + gridDim.x, ..) with the
+// next row's load in flight and its columns' weights in registers.
+template <typename T, typename TW, int VEC, int LANES>
+__global__ void __launch_bounds__(256, 5) forward_kernel(const Fwd p) {
   using R = Raw<T, VEC>;
-  __shared__ float scratch[2][2][32];
-  const int lanes = LANES ? LANES : blockDim.x;
-  const int t = LANES ? threadIdx.x % (LANES ? LANES : 1) : threadIdx.x;
-  const int groups = LANES ? blockDim.x / lanes : 1;       // rows a CTA walks side by side
-  const int64_t stride = (int64_t)gridDim.x * groups;
+  using V = typename Lanes<VEC>::V;
+  constexpr int NP = Lanes<VEC>::N, GROUPS = 256 / LANES;   // rows a CTA walks side by side
+  const int64_t stride = (int64_t)gridDim.x * GROUPS;
   const float inv = 1.0f / (float)p.width;
-  Weights<TW, VEC> w[HELD ? NV : 1], b[HELD ? NV : 1];
-  if constexpr (HELD) {
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int col = (t + k * lanes) * VEC;
-      if (col >= p.width) continue;
-      if (p.w) w[k].load(p.w, col);
-      if (p.b) b[k].load(p.b, col);
-    }
-  }
-  R raw[NV];
+  const int col = threadIdx.x % LANES * VEC;
+  const bool in = col < p.width;
+  Weights<TW, VEC> w, b;
+  if (in && p.w) w.load(p.w, col);
+  if (in && p.b) b.load(p.b, col);
   auto load = [&](int64_t row) {
-    const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int col = (t + k * lanes) * VEC;
-      raw[k] = row < p.rows && col < p.width ? load_once<R>(x + col) : raw_zero<R>();
-    }
+    return in && row < p.rows ? load_once<R>(static_cast<const T*>(p.x) + row * p.x_ld + col) : raw_zero<R>();
   };
-  int64_t row = (int64_t)blockIdx.x * groups + (LANES ? threadIdx.x / lanes : 0);
-  load(row);
-  int half = 0;
-  // Every group takes the same number of turns, so the block's barriers match.
-  for (int64_t base = (int64_t)blockIdx.x * groups; base < p.rows; base += stride, row += stride, half ^= 1) {
-    using V = typename Lanes<VEC>::V;
-    constexpr int NP = Lanes<VEC>::N;
-    V v[NV][NP], acc = vset(V{}, 0.f);
+  int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LANES;
+  R raw = load(row);
+  // Every group takes the same number of turns, so a warp's shuffles match.
+  for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < p.rows; base += stride, row += stride) {
+    V v[NP], acc = vset(V{}, 0.f);
+    unpack_lanes<T, VEC>(raw, v);
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      unpack_lanes<T, VEC>(raw[k], v[k]);
-#pragma unroll
-      for (int i = 0; i < NP; ++i) acc = vadd(acc, v[k][i]);
-    }
-    load(row + stride);
-    const float mean = row_sum<LANES>(hsum(acc), scratch[half]) * inv;
+    for (int i = 0; i < NP; ++i) acc = vadd(acc, v[i]);
+    raw = load(row + stride);
+    const float mean = row_sum<LANES>(hsum(acc), nullptr) * inv;
     const V minus = vset(V{}, -mean);
     acc = vset(V{}, 0.f);
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const bool in = (t + k * lanes) * VEC < p.width;
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        v[k][i] = vadd(v[k][i], minus);
-        if (in) acc = vfma(v[k][i], v[k][i], acc);
-      }
+    for (int i = 0; i < NP; ++i) {
+      v[i] = vadd(v[i], minus);
+      if (in) acc = vfma(v[i], v[i], acc);
     }
-    const float rstd = rsqrtf(row_sum<LANES>(hsum(acc), scratch[half] + 1) * inv + p.eps);
-    if (row >= p.rows) continue;
-    if (t == 0) {
+    const float rstd = rsqrtf(row_sum<LANES>(hsum(acc), nullptr) * inv + p.eps);
+    if (row >= p.rows || !in) continue;
+    if (col == 0) {
       if (p.mean) p.mean[row] = mean;
       if (p.rstd) p.rstd[row] = rstd;
     }
-    T* y = static_cast<T*>(p.y) + row * p.y_ld;
     const V scale = vset(V{}, rstd);
+    V f[NP];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int col = (t + k * lanes) * VEC;
-      if (col >= p.width) continue;
-      V f[NP];
-      if constexpr (!HELD) {
-        if (p.w) w[0].load(p.w, col);
-        if (p.b) b[0].load(p.b, col);
-      }
+    for (int i = 0; i < NP; ++i) v[i] = vmul(v[i], scale);
+    if (p.w) {
+      w.get(f);
 #pragma unroll
-      for (int i = 0; i < NP; ++i) v[k][i] = vmul(v[k][i], scale);
-      if (p.w) {
-        w[HELD ? k : 0].get(f);
-#pragma unroll
-        for (int i = 0; i < NP; ++i) v[k][i] = vmul(v[k][i], f[i]);
-      }
-      if (p.b) {
-        b[HELD ? k : 0].get(f);
-#pragma unroll
-        for (int i = 0; i < NP; ++i) v[k][i] = vadd(v[k][i], f[i]);
-      }
-      store_once(y + col, pack_lanes<T, VEC>(v[k]));
+      for (int i = 0; i < NP; ++i) v[i] = vmul(v[i], f[i]);
     }
+    if (p.b) {
+      b.get(f);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) v[i] = vadd(v[i], f[i]);
+    }
+    store_once(static_cast<T*>(p.y) + row * p.y_ld + col, pack_lanes<T, VEC>(v));
   }
 }
 
@@ -705,11 +672,11 @@ __global__ void __launch_bounds__(256) columns_wide_kernel(const Bwd p) {
 
 constexpr int kSMs = 148;
 
-template <typename T, typename TW, int VEC, int NV, int LANES, int MAXT, int PER_SM, bool HELD>
-static int launch_forward(const Fwd& p, int block, cudaStream_t stream) {
-  const int64_t per = LANES ? block / (LANES ? LANES : 1) : 1;
-  const int64_t ctas = (p.rows + per - 1) / per, most = kSMs * (LANES || block * 2 > MAXT ? PER_SM : 2 * PER_SM);
-  forward_kernel<T, TW, VEC, NV, LANES, MAXT, PER_SM, HELD><<<(unsigned)(ctas < most ? ctas : most), block, 0, stream>>>(p);
+template <typename T, typename TW, int VEC, int LANES>
+static int launch_forward(const Fwd& p, cudaStream_t stream) {
+  constexpr int64_t per = 256 / LANES, most = kSMs * 5;
+  const int64_t ctas = (p.rows + per - 1) / per;
+  forward_kernel<T, TW, VEC, LANES><<<(unsigned)(ctas < most ? ctas : most), 256, 0, stream>>>(p);
   VDN_LAUNCH_CHECK("layer norm");
   return VDN_OK;
 }
@@ -742,11 +709,11 @@ static int forward(const Fwd& p, cudaStream_t stream) {
   const int vec = vector_of<T>(p.width, {p.x_ld, p.y_ld}, {p.x, p.y}, {p.w, p.b}, sizeof(TW));
   const int n = p.width / vec;
   if (vec == V) {
-    if (n <= 8) return launch_forward<T, TW, V, 1, 8, 256, 5, true>(p, 256, stream);
-    if (n <= 16) return launch_forward<T, TW, V, 1, 16, 256, 5, true>(p, 256, stream);
-    if (n <= 32) return launch_forward<T, TW, V, 1, 32, 256, 5, true>(p, 256, stream);
+    if (n <= 8) return launch_forward<T, TW, V, 8>(p, stream);
+    if (n <= 16) return launch_forward<T, TW, V, 16>(p, stream);
+    if (n <= 32) return launch_forward<T, TW, V, 32>(p, stream);
     // 16-bit rows under fp32 weights are bound by the weights' loads: two rows share them.
-    if (sizeof(T) == 2) {
+    if constexpr (sizeof(T) == 2) {
       if (n <= 2 * 32) return launch_row<T, TW, V, 2, 2, 32, 128, 8>(p, 128, stream);
       if (n <= 4 * 32) return launch_row<T, TW, V, 4, 2, 32, 128, 6>(p, 128, stream);
       if (n <= 5 * 256) return launch_row<T, TW, V, 5, 2, 0, 256, 2>(p, (n + 159) / 160 * 32, stream);
@@ -839,11 +806,16 @@ static int backward(const Bwd& p, void* dw, void* db, cudaStream_t stream) {
     else if (n <= 64) rc = launch_backward<T, TW, V, 2, 32, 128, 4, true>(p, 128, lines = few, stream);
     // 16 bits: few fat threads (40 columns, up to 255 registers) cost the fewest instructions a
     // value (5120 columns: 183 us against 227 for 16 columns a thread); 32 bits: bound by HBM
-    else if (M == 1 && n <= 640) rc = launch_ring<T, TW, V, 5, 2, 128, 2, true>(p, (n + 159) / 160 * 32, lines = few_of(ring_lines(p.width)), stream, done);
-    else if (M == 2 && n <= 4 * 320) rc = launch_ring<T, TW, V, 4, 1, 320, 2, true>(p, (n + 127) / 128 * 32, lines, stream, done);
-    else if (n <= 4 * M * 512) rc = launch_ring<T, TW, V, 4 * M, 1, 512, 1, false>(p, (n + 128 * M - 1) / (128 * M) * 32, lines, stream, done);
-    if (n > 64 && n <= 4 * M * 512 && rc == VDN_OK && !done)   // rows too long for two stages
-      rc = launch_backward<T, TW, V, 4 * M, 0, 512, 1, false>(p, (n + 128 * M - 1) / (128 * M) * 32, lines, stream);
+    else if (M == 1 && n <= 640) {
+      if constexpr (M == 1)
+        rc = launch_ring<T, TW, V, 5, 2, 128, 2, true>(p, (n + 159) / 160 * 32, lines = few_of(ring_lines(p.width)), stream, done);
+    } else if (M == 2 && n <= 4 * 320) {
+      if constexpr (M == 2) rc = launch_ring<T, TW, V, 4, 1, 320, 2, true>(p, (n + 127) / 128 * 32, lines, stream, done);
+    } else if (n <= 4 * M * 512) {
+      rc = launch_ring<T, TW, V, 4 * M, 1, 512, 1, false>(p, (n + 128 * M - 1) / (128 * M) * 32, lines, stream, done);
+      if constexpr (M == 2)                          // 32-bit rows too long for two stages (16-bit ones never are)
+        if (rc == VDN_OK && !done) rc = launch_backward<T, TW, V, 4 * M, 0, 512, 1, false>(p, (n + 128 * M - 1) / (128 * M) * 32, lines, stream);
+    }
   } else if (vec == 2) {
     if (n <= 128) rc = launch_backward<T, TW, 2, 4, 32, 128, 4, true>(p, 128, lines = few, stream);
     else if (n <= 8 * 512) rc = launch_backward<T, TW, 2, 8, 0, 512, 1, true>(p, (n + 255) / 256 * 32, lines, stream);
