@@ -408,6 +408,8 @@ int vdn_vda_forward_noalloc(const void* q, const void* k, const void* v, int64_t
  * no other memory with inputs or each other.  zero_tail: write zeros to the rows in
  * front of the first packed sequence and behind the last, else they are left alone.  rows and channels below 2^30, row strides
  * below 2^26.  States and sums are fp32 and added in a fixed order.  status: as in vdn_mxfp8_gemm.
+ * exp(log_decay) counts as 0 below -87.7 and as inf above 88.37; where a product of the decays of up to 256
+ * tokens in a row leaves fp32's range, the state carried in counts as 0 (below) or gives inf or NaN (above).
  * Per-token companion of the frame-wise scan, src/models/linear_attention/scan.py:270-355. */
 int vdn_gated_scan(const void* x, int dtype, int64_t x_batch, int64_t x_row, const void* log_decay,
                    int g_dtype, int64_t g_batch, int64_t g_row, int shared, const float* state,

@@ -22,8 +22,8 @@
 //     for the round's output stores: 480 against 355 us on an early form of the forward
 //     below) this orders nothing else.  No flags in global memory, no workspace, and the
 //     order of every sum is fixed: the same bits on every run.
-// Measured, 16 bits: 1 x 32760 x 5120 forward 270 us (3.7 TB/s), backward 327 (5.1 TB/s); seven
-// packed sequences of 16389 x 5120 backward, an fp32 decay per head, 145 us (3.5 TB/s).  DRAM
+// Measured, 16 bits: 1 x 32760 x 5120 forward 276 us (3.65 TB/s), backward 327 (5.1 TB/s); seven
+// packed sequences of 16389 x 5120 backward, an fp32 decay per head, 133 us (3.8 TB/s).  DRAM
 // and issue slots are half idle: what bounds it is the latency of a round (two walks and the
 // exchange) at the warps that registers and tiles allow.
 //
@@ -116,7 +116,9 @@ __device__ __forceinline__ void unpack_decays(const Raw<TG, GV>& raw, V (&g)[N],
   }
 }
 
-// exp(g) as hi + lo (see above), g clamped: n = round(g / ln 2), r = g - n ln 2, e = expm1(r).
+// exp(g) as hi + lo (see above), g clamped: n = round(g / ln 2) (by adding 1.5 * 2^23, whose neighbours lie 1
+// apart), r = g - n ln 2 with ln 2 in two parts, 355 / 512 and the rest (W. J. Cody and W. Waite, Software Manual
+// for the Elementary Functions, 1980, chapter 6), e = expm1(r).
 template <typename V>
 __device__ __forceinline__ void decay_pair(V g, V& hi, V& lo) {
   auto c = [](float v) { return vset(V{}, v); };
@@ -171,8 +173,8 @@ constexpr int tile_bytes() {   // of one warp and stage: x (dy), the saved y, th
 
 // Tokens a warp.  Runs of 32 keep all their arrays in up to 255 registers and halve the rounds,
 // each of which costs a warp some 250 instructions beside its tokens'; runs of 16 leave room
-// for more warps.  The same whatever the alignment, so that strides do not change the order of
-// the sums.
+// for more warps.  The same for both ways to load rows, so that strides do not change the order of
+// the sums as long as a lane keeps its two channels.
 constexpr int kRun = 16, kLongRun = 32;      // half of that where a lane has four channels
 template <int VEC, int L> constexpr bool long_run() { return L * (VEC == 4 ? 2 : 1) >= kLongRun; }
 
@@ -702,8 +704,9 @@ static void configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, int64_
 // within a tenth of the best of them.  Shared decays cost one evaluation per token instead of
 // one per element: 2 + .. / 4.  Runs of 32 take (2 + the warps) / 4, each scheduler's warps
 // counting as its fullest one's, and no less than 6 / 4: a CTA of six warps on four schedulers
-// takes eight warps' time.  The ring kernel's places decide for both kernels, so that the order
-// of the sums does not hang on alignment.
+// takes eight warps' time.  The ring kernel's places decide for both kernels, so that rows which tensor
+// maps cannot take are summed in the same order; rows that start at an odd element take one channel a
+// lane, and with it a shape of their own.
 template <typename T, typename TG, int VEC, int L, bool BWD, bool SHARED>
 static int choose_shape(int64_t mean, int64_t longest, int64_t seqs, bool sorted, int64_t tiles, int& warps, int& cluster) {
   constexpr int FROM = VEC > 1 || SHARED ? ROWS_UP : ROWS_LOAD;

@@ -232,6 +232,10 @@ def gated_scan(x, log_decay, state=None, *, cu_seqlens=None, reverse=False, out=
     memory is refused.  reverse runs each sequence from
     its last row to its first.  Strided rows and expanded log_decay are read in place as
     long as a row's channels are contiguous.  A state that overflows fp32 comes out as inf or NaN.
+    exp(log_decay) counts as 0 below -87.7 and as inf above 88.37.  Decays may grow (log_decay above 0), but up to
+    256 tokens in a row are folded into one factor: where a product of successive decays among them leaves
+    fp32's range, the state carried in counts as 0 (below the range) or gives inf or NaN (above), even if the
+    states themselves would have stayed inside.
     """
     if torch.is_grad_enabled() and _lib.records(x, log_decay, state, out, out_state):
         if out is not None or out_state is not None:
