@@ -95,6 +95,10 @@ def test_columns_of_one_buffer(cuda):
     turned = buffer.transpose(0, 1).contiguous().transpose(0, 1)       # token-major
     part = [turned[..., i * 128:(i + 1) * 128].unflatten(-1, (2, 64)) for i in range(5)]
     assert torch.equal(gated_scan(part[0], part[2], state, out=part[4])[0], want[0])
+    for buffer in (torch.zeros(4, 40, 2, 64, device=cuda), torch.zeros(2, 80, 2, 64, device=cuda)):
+        part = [buffer[i::2] if len(buffer) == 4 else buffer[:, i::2] for i in range(2)]    # every other batch, every other row
+        part[1].copy_(x)
+        assert torch.equal(gated_scan(part[1], g, state, out=part[0])[0], want[0])
     one = [t[:, :1] for t in (x, g)]                                   # a step keeps its state in its output
     want = gated_scan(*one, state)
     hold = state.clone()

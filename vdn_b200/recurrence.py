@@ -120,16 +120,22 @@ def _same(a, b):
 
 
 def _beside(a, b, lead):
-    """Whether a's and b's rows are different columns of rows of one buffer: no address in both."""
-    steps = [(p, q) for n, p, q in zip(a.shape[:lead], a.stride(), b.stride()) if n > 1]
-    if not steps or a.element_size() != b.element_size() or a.shape[:lead] != b.shape[:lead]:
+    """Whether a and b, rows of one buffer at the same strides, are different parts of each of its periods
+    (columns of the same rows, every other row, every other batch): no address in both."""
+    if a.element_size() != b.element_size() or a.shape[:lead] != b.shape[:lead]:
         return False
-    pitch = min(p for p, _ in steps)
-    wide, narrow = a.shape[lead:].numel(), b.shape[lead:].numel()
-    if pitch < 1 or any(p != q or p % pitch for p, q in steps):
+    dims = sorted((q, n) for n, p, q in zip(a.shape[:lead], a.stride(), b.stride()) if n > 1 and p == q)
+    if len(dims) != sum(n > 1 for n in a.shape[:lead]):
         return False
-    off = (b.data_ptr() - a.data_ptr()) // a.element_size() % pitch
-    return off >= wide and off + narrow <= pitch
+    off = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    inner = 0                                         # what the smaller strides span
+    for i, (pitch, n) in enumerate(dims):
+        if pitch > 0 and all(p % pitch == 0 for p, _ in dims[i:]):
+            first = off % pitch
+            if first >= inner + a.shape[lead:].numel() and first + inner + b.shape[lead:].numel() <= pitch:
+                return True
+        inner += (n - 1) * pitch
+    return False
 
 
 def _check_memory(x, log_decay, state, out, out_state, lead):
