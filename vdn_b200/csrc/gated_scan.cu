@@ -22,7 +22,7 @@
 //     for the round's output stores: 480 against 355 us on an early form of the forward
 //     below) this orders nothing else.  No flags in global memory, no workspace, and the
 //     order of every sum is fixed: the same bits on every run.
-// Measured, 16 bits: 1 x 32760 x 5120 forward 276 us (3.65 TB/s), backward 327 (5.1 TB/s); seven
+// Measured, 16 bits: 1 x 32760 x 5120 forward 276 us (3.65 TB/s), backward 334 (5.0 TB/s); seven
 // packed sequences of 16389 x 5120 backward, an fp32 decay per head, 133 us (3.8 TB/s).  DRAM
 // and issue slots are half idle: what bounds it is the latency of a round (two walks and the
 // exchange) at the warps that registers and tiles allow.
