@@ -3,8 +3,8 @@
 With u = 2^-24.  The decay is a pair hi + lo within 2.5e-8 = 0.42u of exp(g), relative.  A step rounds twice
 (x + lo h, then hi h + that: u/2 each of values at most M_t, the recurrence on absolute values).  A carry reaches token l
 through the product of the hi parts (0.42u, u/2 for hi and u/2 for the product a token).  Joining a warp's run of
-16 or 32 tokens and a CTA's run of up to 256 rounds some six times more, and the run's factor errs by the rounding of its
-sum of decays, n u/2 |S| exp(S) <= 0.19 n u.  Together below 3u M_t a token."""
+16 or 32 tokens and a CTA's run of up to 256 rounds some six times more, and the run's factor errs by at most u a
+token, whether it comes from the sum of its decays (at most 2) or from their product.  Together below 3u M_t a token."""
 import pytest
 import torch
 

@@ -22,7 +22,7 @@
 //     for the round's output stores: 480 against 355 us on an early form of the forward
 //     below) this orders nothing else.  No flags in global memory, no workspace, and the
 //     order of every sum is fixed: the same bits on every run.
-// Measured, 16 bits: 1 x 32760 x 5120 forward 276 us (3.65 TB/s), backward 334 (5.0 TB/s); seven
+// Measured, 16 bits: 1 x 32760 x 5120 forward 270 us (3.7 TB/s), backward 330 (5.1 TB/s); seven
 // packed sequences of 16389 x 5120 backward, an fp32 decay per head, 133 us (3.8 TB/s).  DRAM
 // and issue slots are half idle: what bounds it is the latency of a round (two walks and the
 // exchange) at the warps that registers and tiles allow.
@@ -32,9 +32,9 @@
 // the same way at every token), so exp(g) is kept as a pair hi + lo with 2^n as a common
 // factor: hi = fp32(1 + e), lo = e - (hi - 1), e = expm1(r) with r = g - n ln 2 in [-0.35,
 // 0.35] from a polynomial fitted at Chebyshev nodes (2.5e-8 relative).  It runs on packed
-// fp32 pairs with no branch and no MUFU operation.  A run's A comes from the sum of its g, not
-// from the product of its rounded decays; the sum takes g before it is clamped, so that a -inf stays one
-// however much growth stands beside it.  exp(g) is 0 below g = -87.7 and inf above 88.37.
+// fp32 pairs with no branch and no MUFU operation.  A run's A comes from the sum of its g where
+// that lies in [-2, 2], else from the product of its decays (run_factor).  exp(g) is 0 below g = -87.7 and inf
+// above 88.37.
 #include <initializer_list>
 #include <type_traits>
 
@@ -101,18 +101,20 @@ template <> __device__ __forceinline__ uint32_t clamp_word<__half>(uint32_t w) {
   asm("{\n\t.reg .b32 t;\n\tmax.NaN.f16x2 t, %1, %2;\n\tmin.NaN.f16x2 %0, t, %3;\n\t}" : "=r"(r) : "r"(w), "r"(0xD57ED57Eu), "r"(0x55885588u));
   return r;
 }
-// The log decays as they are, for a run's sum (a -inf must stay one beside growth), and held.
 template <typename TG, int GV, typename V, int N>
-__device__ __forceinline__ void unpack_decays(const Raw<TG, GV>& raw, V (&g)[N], V (&held)[N]) {
-  unpack_lanes<TG, GV>(raw, g);
+__device__ __forceinline__ void unpack_decays(const Raw<TG, GV>& raw, V (&g)[N]) {
   if constexpr (GV * sizeof(TG) < 4) {
-    held[0] = clamp_decay(g[0]);
+    float e[1];
+    unpack<TG, 1>(raw, e);
+    e[0] = clamp_decay(e[0]);
+    to_lanes(e, g);
   } else {
     uint32_t w[GV * sizeof(TG) / 4];
     words(raw, w);
 #pragma unroll
     for (auto& x : w) x = clamp_word<TG>(x);
-    unpack_lanes<TG, GV>(join(w), held);
+    const auto held = join(w);
+    unpack_lanes<TG, GV>(held, g);
   }
 }
 
@@ -140,6 +142,21 @@ __device__ __forceinline__ V decay_of(V g) {         // of any g
   V hi, lo;
   decay_pair(clamp_decay(g), hi, lo);
   return vadd(hi, lo);
+}
+
+// The factor of a CTA's run from the sum s of its log decays or the product p of their hi parts.  The product
+// errs by u a token (u = 2^-24), all in one direction where the decays are alike, and slow decays remember that over
+// many runs; the sum's exponential errs by half a unit of s an addition, 32 u at s = -62, which tells where little
+// of the carry is left.  At |s| = 2 the product's errors leave at most 256 u / (e^2 - 1) = 40 u in a stationary state.
+// A product of 0 stands: some decay was 0 (the sum holds it as -87.9, and growth beside it would cancel that).
+__device__ __forceinline__ float run_factor(float s, float p, float e) { return fabsf(s) <= 2.f && p != 0.f ? e : p; }
+__device__ __forceinline__ float run_factor(float s, float p) { return run_factor(s, p, decay_of(s)); }
+__device__ __forceinline__ f2 run_factor(f2 s, f2 p) {
+  float s0, s1, p0, p1, e0, e1;
+  f2_unpack(s, s0, s1);
+  f2_unpack(p, p0, p1);
+  f2_unpack(decay_of(s), e0, e1);
+  return f2_pack(run_factor(s0, p0, e0), run_factor(s1, p1, e1));
 }
 
 // A run's map c -> a c + h.
@@ -374,8 +391,8 @@ __global__ void __launch_bounds__(max_warps<T, TG, VEC, L, BWD, SHARED>() * 32, 
     }
     float hi_lane = 1.f, lo_lane = 0.f;
     if constexpr (SHARED) {
-      decay_pair(clamp_decay(g_next), hi_lane, lo_lane);
-      float s = g_next;
+      float s = clamp_decay(g_next);                 // not at the load: nothing waits for it there
+      decay_pair(s, hi_lane, lo_lane);
 #pragma unroll
       for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       sum[0] = vset(G{}, s);
@@ -385,18 +402,18 @@ __global__ void __launch_bounds__(max_warps<T, TG, VEC, L, BWD, SHARED>() * 32, 
 #pragma unroll
       for (int l = 0; l < L; ++l) {
         V x[NV];
-        G g[NG], held[NG], hi[NG], lo[NG];
+        G g[NG], hi[NG], lo[NG];
         unpack_lanes<T, VEC>(RING ? *x_at(l) : rx[RING ? 0 : l], x);
         if constexpr (SHARED) {
           hi[0] = vset(G{}, __shfl_sync(0xffffffffu, hi_lane, l));
           lo[0] = vset(G{}, __shfl_sync(0xffffffffu, lo_lane, l));
         } else {
-          unpack_decays<TG, GV>(RING ? *g_at(l) : rg[RING || SHARED ? 0 : l], g, held);
+          unpack_decays<TG, GV>(RING ? *g_at(l) : rg[RING || SHARED ? 0 : l], g);
         }
 #pragma unroll
         for (int v = 0; v < NG; ++v) {
           if constexpr (!SHARED) {
-            decay_pair(held[v], hi[v], lo[v]);
+            decay_pair(g[v], hi[v], lo[v]);
             sum[v] = vadd(sum[v], g[v]);
           }
           far[v] = vmul(far[v], hi[v]);
@@ -423,7 +440,7 @@ __global__ void __launch_bounds__(max_warps<T, TG, VEC, L, BWD, SHARED>() * 32, 
     }
 
     // Join the warps of the CTA: `before` is the fold of the warps in front of this one.
-    // (Inside a round the product of the run's decays will do; the sums carry the long chain.)
+    // (Inside a round the product of the run's decays will do; run_factor chooses for the long chain.)
     Fold<V> own[NV], before[NV];
 #pragma unroll
     for (int v = 0; v < NG; ++v) sums[buf][warp][v][lane] = sum[v];
@@ -456,11 +473,20 @@ __global__ void __launch_bounds__(max_warps<T, TG, VEC, L, BWD, SHARED>() * 32, 
         for (int v = 0; v < NG; ++v) s[v] = vadd(s[v], sums[buf][w][v][lane]);
       }
 #pragma unroll
-      for (int v = 0; v < NG; ++v) s[v] = decay_of(s[v]);
-#pragma unroll
       for (int v = 0; v < NV; ++v) {
         Fold<V> f;
-        spread(s[SHARED ? 0 : v], f.a);
+        if constexpr (SHARED) {
+          float p;                                   // one decay for the whole head
+          if constexpr (std::is_same<V, float>::value) {
+            p = before[v].a * own[v].a;
+          } else {
+            float unused;
+            f2_unpack(vmul(before[v].a, own[v].a), p, unused);
+          }
+          spread(run_factor(s[0], p), f.a);
+        } else {
+          f.a = run_factor(s[v], vmul(before[v].a, own[v].a));
+        }
         f.h = vfma(own[v].a, before[v].h, own[v].h);
         for (int r = 0; r < cluster; ++r)
           send(mapa_shared(&runs[buf][rank][v][lane], r), f, mapa_shared(&arrived[buf], r));
